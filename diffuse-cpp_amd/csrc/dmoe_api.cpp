@@ -20,6 +20,7 @@
 #include <vector>
 
 #include "dmoe_internal.h"
+#include "dmoe_kv_plan.h"
 
 using namespace dmoe;
 
@@ -1699,22 +1700,22 @@ size_t plan_attn(const KernelSwitches &sw, const dmoe_layer *L, int N, bool host
     return off;
 }
 
-int enqueue_attn(dmoe_ctx *ctx, const dmoe_layer *L, const AttnWs &w, const float *h, int N, float *h_out,
-                 float *moe_in, hipStream_t s)
+// Input norm and fused QKV projection of h into *qkv (qks reduction slices,
+// N QKV floats apart).
+int enqueue_attn_qkv(dmoe_ctx *ctx, const dmoe_layer *L, const AttnWs &w, const float *h, int N, const float **qkv,
+                     int *qks, hipStream_t s)
 {
     const dmoe_attn_hparams &a = L->ahp;
     const int H = a.n_embd, QD = a.n_head * a.head_dim, KD = a.n_head_kv * a.head_dim, QKV = QD + 2 * KD;
     const bool prof = ctx->prof;
     // projections on the few-token kernel or the GEMM: the norms
     // hand them int8 digits and take their reduction slices directly
-    // (k_norm_fused, k_qk_rope)
+    // (k_norm_fused, k_qk_rope, k_kv_append)
     const bool fq = proj_takes_digits(w.pq, N) && H <= 8192;
-    const bool fo = proj_takes_digits(w.po, N) && H <= 8192;
 #define STAGE(id, call) LAUNCH_TRY(ctx, stage(ctx, prof, id, s, [&] { return call; }))
     // :120-121 input layernorm; :124 fused QKV
-    const float *qkv = w.qkv;
-    int qks = 1;
-    int rc;
+    *qkv = w.qkv;
+    *qks = 1;
     if (fq) {
         NormArgs na{};
         na.h_in = h;
@@ -1724,29 +1725,24 @@ int enqueue_attn(dmoe_ctx *ctx, const dmoe_layer *L, const AttnWs &w, const floa
         na.H = H;
         na.eps = a.rms_eps;
         STAGE(ST_FRONT, launch_norm_fused(na, s));
-        if ((rc = enqueue_proj_digits(ctx, prof, ST_SH_GATEUP, L->aqkv, QKV, H, N, w.pq, w.qkv, &qks, &qkv, s)))
-            return rc;
-    } else {
-        STAGE(ST_FRONT, launch_residual_rmsnorm(const_cast<float *>(h), nullptr, L->attn_norm, w.xn, N, H,
-                                                a.rms_eps, s));
-        if ((rc = enqueue_proj(ctx, prof, ST_ACTQ_X, ST_SH_GATEUP, L->aqkv, QKV, H, w.xn, N, w.qkv, w.pq, s)))
-            return rc;
+        return enqueue_proj_digits(ctx, prof, ST_SH_GATEUP, L->aqkv, QKV, H, N, w.pq, w.qkv, qks, qkv, s);
     }
-    AttnDims d{};
-    d.n = N;
-    d.nh = a.n_head;
-    d.nkv = a.n_head_kv;
-    d.hd = a.head_dim;
-    d.rd = a.rotary_dim;
-    d.qk_norm = a.use_qk_norm;
-    d.block = a.block_length;
-    d.eps = a.rms_eps;
-    // the rope cache's angle step, as ggml computes it on the host
-    d.theta_scale = a.rotary_dim > 0 ? powf(a.rope_base, -2.0f / (float)a.rotary_dim) : 1.0f;
-    d.scale = 1.0f / sqrtf((float)a.head_dim);
-    d.waves = ctx->sw.attn_waves;
-    STAGE(ST_ROUTE, launch_qk_rope(qkv, qks, (size_t)N * QKV, L->qn, L->kn, d, w.Qh, w.Kh, w.Vh, s));
-    STAGE(ST_SCORES, launch_attn(w.Qh, w.Kh, w.Vh, d, w.att, s));
+    STAGE(ST_FRONT, launch_residual_rmsnorm(const_cast<float *>(h), nullptr, L->attn_norm, w.xn, N, H,
+                                            a.rms_eps, s));
+#undef STAGE
+    return enqueue_proj(ctx, prof, ST_ACTQ_X, ST_SH_GATEUP, L->aqkv, QKV, H, w.xn, N, w.qkv, w.pq, s);
+}
+
+// Output projection of w.att, residual and post-attention norm.
+int enqueue_attn_out(dmoe_ctx *ctx, const dmoe_layer *L, const AttnWs &w, const float *h, int N, float *h_out,
+                     float *moe_in, hipStream_t s)
+{
+    const dmoe_attn_hparams &a = L->ahp;
+    const int H = a.n_embd, QD = a.n_head * a.head_dim;
+    const bool prof = ctx->prof;
+    const bool fo = proj_takes_digits(w.po, N) && H <= 8192;
+    int rc;
+#define STAGE(id, call) LAUNCH_TRY(ctx, stage(ctx, prof, id, s, [&] { return call; }))
     // :172 output projection; :175-178 residual, then the post-attention
     // layernorm (the MoE input)
     if (fo) {
@@ -1777,6 +1773,182 @@ int enqueue_attn(dmoe_ctx *ctx, const dmoe_layer *L, const AttnWs &w, const floa
     }
 #undef STAGE
     return DMOE_OK;
+}
+
+int enqueue_attn(dmoe_ctx *ctx, const dmoe_layer *L, const AttnWs &w, const float *h, int N, float *h_out,
+                 float *moe_in, hipStream_t s)
+{
+    const dmoe_attn_hparams &a = L->ahp;
+    const int QKV = (a.n_head + 2 * a.n_head_kv) * a.head_dim;
+    const bool prof = ctx->prof;
+    const float *qkv;
+    int qks;
+    const int rc = enqueue_attn_qkv(ctx, L, w, h, N, &qkv, &qks, s);
+    if (rc) return rc;
+#define STAGE(id, call) LAUNCH_TRY(ctx, stage(ctx, prof, id, s, [&] { return call; }))
+    AttnDims d{};
+    d.n = N;
+    d.nh = a.n_head;
+    d.nkv = a.n_head_kv;
+    d.hd = a.head_dim;
+    d.rd = a.rotary_dim;
+    d.qk_norm = a.use_qk_norm;
+    d.block = a.block_length;
+    d.eps = a.rms_eps;
+    // the rope cache's angle step, as ggml computes it on the host
+    d.theta_scale = a.rotary_dim > 0 ? powf(a.rope_base, -2.0f / (float)a.rotary_dim) : 1.0f;
+    d.scale = 1.0f / sqrtf((float)a.head_dim);
+    d.waves = ctx->sw.attn_waves;
+    STAGE(ST_ROUTE, launch_qk_rope(qkv, qks, (size_t)N * QKV, L->qn, L->kn, d, w.Qh, w.Kh, w.Vh, s));
+    STAGE(ST_SCORES, launch_attn(w.Qh, w.Kh, w.Vh, d, w.att, s));
+#undef STAGE
+    return enqueue_attn_out(ctx, L, w, h, N, h_out, moe_in, s);
+}
+
+// ---------------------------------------------------------------------------
+// The paged KV cache.
+
+// Restores the caller's current device.
+struct DeviceGuard {
+    int before = -1;
+    ~DeviceGuard()
+    {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    hipError_t use(int device)
+    {
+        int now = 0;
+        hipError_t e = hipGetDevice(&now);
+        if (e != hipSuccess || now == device) return e;
+        e = hipSetDevice(device);
+        if (e == hipSuccess) before = now;
+        return e;
+    }
+};
+
+// Whether `s` is being captured into a graph.
+hipError_t capturing(hipStream_t s, bool *yes)
+{
+    *yes = false;
+    if (!s) return hipSuccess;           // the null stream cannot be captured
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing(s, &st);
+    *yes = st == hipStreamCaptureStatusActive;
+    return e;
+}
+
+int refuse(dmoe_ctx *ctx, const KvRefusal &r) { return set_err(ctx, r.code, "%s", r.why); }
+
+KvCacheView kv_view(const dmoe_kv_cache &kv)
+{
+    return KvCacheView{kv.type, kv.page_tokens, kv.n_pages, kv.k, kv.v, kv.k_exp, kv.v_exp};
+}
+
+KvBatch kv_batch(const dmoe_kv_batch &b)
+{
+    return KvBatch{b.n_seqs, b.n_tokens, b.max_pages, b.q_start, b.kv_len, b.pages};
+}
+
+KvAppendArgs kv_append_args(const dmoe_kv_cache &kv, const dmoe_kv_batch &b, const dmoe_attn_hparams &a,
+                            const float *q_norm, const float *k_norm)
+{
+    KvAppendArgs k{};
+    k.c = kv_view(kv);
+    k.b = kv_batch(b);
+    k.nh = a.n_head;
+    k.nkv = a.n_head_kv;
+    k.hd = a.head_dim;
+    k.rd = a.rotary_dim;
+    k.qk_norm = a.use_qk_norm != 0;
+    k.eps = a.rms_eps;
+    k.log2_step = a.rotary_dim > 0 ? -2.0 * std::log2((double)a.rope_base) / a.rotary_dim : 0.0;
+    k.ks = 1;
+    k.q_norm = q_norm;
+    k.k_norm = k_norm;
+    return k;
+}
+
+KvAttnArgs kv_attn_args(const dmoe_kv_cache &kv, const dmoe_kv_batch &b, const dmoe_attn_hparams &a)
+{
+    KvAttnArgs k{};
+    k.c = kv_view(kv);
+    k.b = kv_batch(b);
+    k.nh = a.n_head;
+    k.nkv = a.n_head_kv;
+    k.hd = a.head_dim;
+    k.block = a.block_length;
+    k.scale = 1.0f / sqrtf((float)a.head_dim);
+    return k;
+}
+
+// The workspace of a cached call: the caller's, or the context's own (which a
+// captured call may not use: a later call that grows it would free what the
+// graph holds).
+int kv_workspace(dmoe_ctx *ctx, void *ws, size_t bytes, size_t need, hipStream_t s, uint8_t **out)
+{
+    if (ws) {
+        KvRefusal r;
+        if (kv_check_workspace(r, ws, bytes, need)) return refuse(ctx, r);
+        *out = (uint8_t *)ws;
+        return DMOE_OK;
+    }
+    bool graph = false;
+    HIP_TRY(ctx, capturing(s, &graph));
+    if (graph) return set_err(ctx, DMOE_ERR_INVALID_ARG, "kv: a captured call needs a workspace of its own (%zu bytes)", need);
+    const int rc = grow_workspace(ctx, need);
+    *out = (uint8_t *)ctx->ws;
+    return rc;
+}
+
+// plan_attn's buffers for the cached half: queries token-major, no keys and
+// values of its own.
+size_t plan_attn_cached(const KernelSwitches &sw, const dmoe_layer *L, const dmoe_kv_cache &kv, const dmoe_kv_batch &b,
+                        uint8_t *base, AttnWs *w, void **kv_ws)
+{
+    const dmoe_attn_hparams &a = L->ahp;
+    const int H = a.n_embd, QD = a.n_head * a.head_dim, QKV = QD + 2 * a.n_head_kv * a.head_dim, N = b.n_tokens;
+    size_t off = 0;
+    auto take = [&](size_t bytes) -> uint8_t * {
+        uint8_t *p = base ? base + off : nullptr;
+        off += align_up(bytes > 0 ? bytes : 1);
+        return p;
+    };
+    AttnWs t{};
+    t.xn = (float *)take((size_t)N * H * 4);
+    t.qkv = (float *)take((size_t)N * QKV * 4);
+    t.Qh = (float *)take((size_t)N * QD * 4);
+    t.att = (float *)take((size_t)N * QD * 4);
+    t.proj = (float *)take((size_t)N * H * 4);
+    t.scratch = (float *)take((size_t)N * H * 4);
+    t.pq = plan_proj(sw, head_path(L->aqkv.type, QKV, H), N, H, QKV, take);
+    t.po = plan_proj(sw, head_path(L->awo.type, H, QD), N, QD, H, take);
+    void *k = take(kv_attn_ws_bytes(kv_attn_args(kv, b, a)));
+    if (w) *w = t;
+    if (kv_ws) *kv_ws = k;
+    return off;
+}
+
+int enqueue_attn_cached(dmoe_ctx *ctx, const dmoe_layer *L, const AttnWs &w, void *kv_ws, const dmoe_kv_cache &kv,
+                        const dmoe_kv_batch &b, const float *h, float *h_out, float *moe_in, hipStream_t s)
+{
+    const dmoe_attn_hparams &a = L->ahp;
+    const int N = b.n_tokens;
+    const bool prof = ctx->prof;
+    KvAppendArgs ka = kv_append_args(kv, b, a, L->qn, L->kn);
+    const int rc = enqueue_attn_qkv(ctx, L, w, h, N, &ka.qkv, &ka.ks, s);
+    if (rc) return rc;
+    ka.kstride = (size_t)N * (a.n_head + 2 * a.n_head_kv) * a.head_dim;
+    ka.q_out = w.Qh;
+    ka.rest = w.att;
+    KvAttnArgs at = kv_attn_args(kv, b, a);
+    at.q = w.Qh;
+    at.out = w.att;
+    at.ws = kv_ws;
+#define STAGE(id, call) LAUNCH_TRY(ctx, stage(ctx, prof, id, s, [&] { return call; }))
+    STAGE(ST_ROUTE, launch_kv_append(ka, s));
+    STAGE(ST_SCORES, launch_kv_attn(at, s));
+#undef STAGE
+    return enqueue_attn_out(ctx, L, w, h, N, h_out, moe_in, s);
 }
 
 } // namespace
@@ -2203,6 +2375,94 @@ int dmoe_attn_forward_device(dmoe_ctx *ctx, const dmoe_layer *L, const float *h_
     AttnWs w;
     plan_attn(ctx->sw, L, n_tokens, false, (uint8_t *)ctx->ws, &w);
     return enqueue_attn(ctx, L, w, h_dev, n_tokens, h_out_dev, moe_in_dev, (hipStream_t)stream);
+}
+
+int dmoe_kv_append_device(dmoe_ctx *ctx, const dmoe_kv_cache *kv, const dmoe_kv_batch *batch,
+                          const dmoe_attn_hparams *ap, const float *qkv_dev, const float *q_norm_dev,
+                          const float *k_norm_dev, float *q_out_dev, void *stream)
+{
+    if (!ctx) return DMOE_ERR_INVALID_ARG;
+    KvRefusal r;
+    if (kv_check_append(r, kv, batch, ap, qkv_dev, q_norm_dev, k_norm_dev, q_out_dev)) return refuse(ctx, r);
+    DeviceGuard device;
+    HIP_TRY(ctx, device.use(ctx->device));
+    KvAppendArgs a = kv_append_args(*kv, *batch, *ap, q_norm_dev, k_norm_dev);
+    a.qkv = qkv_dev;
+    a.q_out = q_out_dev;
+    LAUNCH_TRY(ctx, launch_kv_append(a, (hipStream_t)stream));
+    return DMOE_OK;
+}
+
+size_t dmoe_kv_attn_workspace(dmoe_ctx *ctx, const dmoe_kv_cache *kv, const dmoe_kv_batch *batch,
+                              const dmoe_attn_hparams *ap)
+{
+    KvRefusal r;
+    if (!ctx) return 0;
+    if (kv_check(r, kv, batch, ap, false)) {
+        refuse(ctx, r);
+        return 0;
+    }
+    return kv_attn_ws_bytes(kv_attn_args(*kv, *batch, *ap));
+}
+
+int dmoe_kv_attn_device(dmoe_ctx *ctx, const dmoe_kv_cache *kv, const dmoe_kv_batch *batch,
+                        const dmoe_attn_hparams *ap, const float *q_dev, float *out_dev, void *workspace_dev,
+                        size_t workspace_bytes, void *stream)
+{
+    if (!ctx) return DMOE_ERR_INVALID_ARG;
+    KvRefusal r;
+    if (kv_check_attn(r, kv, batch, ap, q_dev, out_dev)) return refuse(ctx, r);
+    DeviceGuard device;
+    HIP_TRY(ctx, device.use(ctx->device));
+    KvAttnArgs a = kv_attn_args(*kv, *batch, *ap);
+    a.q = q_dev;
+    a.out = out_dev;
+    uint8_t *ws = nullptr;
+    const int rc = kv_workspace(ctx, workspace_dev, workspace_bytes, kv_attn_ws_bytes(a), (hipStream_t)stream, &ws);
+    if (rc) return rc;
+    a.ws = ws;
+    LAUNCH_TRY(ctx, launch_kv_attn(a, (hipStream_t)stream));
+    return DMOE_OK;
+}
+
+static int attn_cached_layer(dmoe_ctx *ctx, const dmoe_layer *L)
+{
+    if (!L || !L->attn) return set_err(ctx, DMOE_ERR_INVALID_ARG, "not an attention layer (dmoe_attn_upload)");
+    if (L->device != ctx->device)
+        return set_err(ctx, DMOE_ERR_INVALID_ARG, "layer lives on device %d, context on %d", L->device, ctx->device);
+    return DMOE_OK;
+}
+
+size_t dmoe_attn_cached_workspace(dmoe_ctx *ctx, const dmoe_layer *attn, const dmoe_kv_cache *kv,
+                                  const dmoe_kv_batch *batch)
+{
+    KvRefusal r;
+    if (!ctx || attn_cached_layer(ctx, attn)) return 0;
+    if (kv_check(r, kv, batch, &attn->ahp, false)) {
+        refuse(ctx, r);
+        return 0;
+    }
+    return plan_attn_cached(ctx->sw, attn, *kv, *batch, nullptr, nullptr, nullptr);
+}
+
+int dmoe_attn_forward_cached_device(dmoe_ctx *ctx, const dmoe_layer *attn, const dmoe_kv_cache *kv,
+                                    const dmoe_kv_batch *batch, const float *h_dev, float *h_out_dev,
+                                    float *moe_in_dev, void *workspace_dev, size_t workspace_bytes, void *stream)
+{
+    if (!ctx) return DMOE_ERR_INVALID_ARG;
+    int rc = attn_cached_layer(ctx, attn);
+    if (rc) return rc;
+    KvRefusal r;
+    if (kv_check_layer(r, kv, batch, &attn->ahp, h_dev, h_out_dev, moe_in_dev)) return refuse(ctx, r);
+    DeviceGuard device;
+    HIP_TRY(ctx, device.use(ctx->device));
+    const size_t need = plan_attn_cached(ctx->sw, attn, *kv, *batch, nullptr, nullptr, nullptr);
+    uint8_t *ws = nullptr;
+    if ((rc = kv_workspace(ctx, workspace_dev, workspace_bytes, need, (hipStream_t)stream, &ws))) return rc;
+    AttnWs w;
+    void *kv_ws = nullptr;
+    plan_attn_cached(ctx->sw, attn, *kv, *batch, ws, &w, &kv_ws);
+    return enqueue_attn_cached(ctx, attn, w, kv_ws, *kv, *batch, h_dev, h_out_dev, moe_in_dev, (hipStream_t)stream);
 }
 
 int dmoe_dense_upload(dmoe_ctx *ctx, int32_t n_embd, int32_t n_ff, const dmoe_tensor *gate,

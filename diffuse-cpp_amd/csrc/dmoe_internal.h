@@ -233,6 +233,44 @@ hipError_t launch_qk_rope(const float *qkv, int ks, size_t kstride, const float 
 // block-causal GQA attention -> out [N][nh hd]
 hipError_t launch_attn(const float *Qh, const float *Kh, const float *Vh, const AttnDims &a, float *out,
                        hipStream_t s);
+// The paged KV cache (dmoe_kv.h has its layout; k_kv_append.hip, k_kv_attn.hip).
+constexpr int KV_EMIN = -50, KV_EMAX = 50;   // exponents of an E4M3 block
+struct KvCacheView {
+    int32_t type, T, n_pages;            // DMOE_KV_*, tokens a page, pages
+    void *k, *v;
+    int8_t *k_exp, *v_exp;
+};
+struct KvBatch {
+    int32_t n_seqs, n_tokens, max_pages;
+    const int32_t *q_start, *kv_len, *pages;
+};
+struct KvAppendArgs {
+    KvCacheView c;
+    KvBatch b;
+    int32_t nh, nkv, hd, rd, qk_norm;
+    float eps;
+    double log2_step;                    // log2 of the frequencies' ratio: -2 log2(base) / rd
+    const float *qkv;                    // fused rows: the sum of ks slices kstride floats apart
+    int32_t ks;
+    size_t kstride;
+    const float *q_norm, *k_norm;
+    float *q_out;                        // [n_tokens][nh][hd]
+    float *rest;                         // when given: rows of [n_tokens][nh][hd] past the last sequence's to zero
+    int32_t blocks;                      // set by the launch
+};
+hipError_t launch_kv_append(const KvAppendArgs &a, hipStream_t s);
+struct KvAttnArgs {
+    KvCacheView c;
+    KvBatch b;
+    int32_t nh, nkv, hd, block;
+    float scale;                         // 1 / sqrt(hd)
+    const float *q;                      // [n_tokens][nh][hd]
+    float *out;
+    void *ws;
+};
+hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t s);
+// bytes of a.ws that the launch needs; the tables are not read
+size_t kv_attn_ws_bytes(const KvAttnArgs &a);
 // Per row of V logits: the argmax (first index of the largest) and its
 // softmax probability 1 / sum exp(l - max) (k_head.hip), through per-chunk
 // partials (argmax_partials_bytes of workspace).

@@ -1,0 +1,77 @@
+// dmoe_kv.h — the paged KV cache as its kernels see it (k_kv_append.hip,
+// k_kv_attn.hip) and the device helpers that both use.
+//
+// Layouts, T tokens a page, blocks of 32 tokens, 16-byte pieces:
+//   k  [n_pages][nkv][T][hd]
+//   v  [n_pages][nkv][T / 32] blocks, transposed so that a lane's operand of
+//      the P V product (8 consecutive tokens of a dim) is one piece (F16) or
+//      half of one (E4M3):
+//        F16   piece 4 d + t / 8: tokens t .. t + 7 (t % 8 == 0) of dim d
+//        E4M3  piece 4 (d / 2) + t / 8: tokens t .. t + 7 of dim d, then of d + 1
+//   k_exp, v_exp  int8 [n_pages][nkv][T / 32]: a block's values are code * 2^exp
+#pragma once
+
+#include "dmoe_internal.h"
+#include "dmoe_kv_plan.h"
+
+namespace dmoe {
+
+typedef _Float16 kv_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 kv_h2 __attribute__((ext_vector_type(2)));
+typedef float kv_f4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ KvSeq kv_seq(const KvBatch &b, int s)
+{
+    return kv_seq_of(b.q_start[s], b.q_start[s + 1], b.kv_len[s], b.n_tokens);
+}
+
+// Inclusive prefix sum over the 64 lanes.
+__device__ __forceinline__ int kv_wave_scan(int v)
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int u = __shfl_up(v, d, 64);
+        if (lane >= d) v += u;
+    }
+    return v;
+}
+
+// Item `item` of a list that holds count(seq) items of each sequence in turn:
+// its sequence (and the item's index within it), found by one wavefront in
+// steps of 64 sequences; false past the list's end.
+template <class Count>
+__device__ __forceinline__ bool kv_find(const KvBatch &b, int item, Count &&count, int &seq, KvSeq &info, int &index)
+{
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < b.n_seqs; base += 64) {
+        KvSeq q{0, 0, 0};
+        int c = 0;
+        if (base + lane < b.n_seqs) {
+            q = kv_seq(b, base + lane);
+            c = count(q);
+        }
+        const int end = kv_wave_scan(c);
+        const uint64_t past = __ballot(end > item);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            seq = base + l;
+            info.q0 = __builtin_amdgcn_readlane(q.q0, l);
+            info.n = __builtin_amdgcn_readlane(q.n, l);
+            info.len = __builtin_amdgcn_readlane(q.len, l);
+            index = item - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(c, l));
+            return true;
+        }
+        item -= __builtin_amdgcn_readlane(end, 63);
+    }
+    return false;
+}
+
+// The page that holds token `pos` of sequence s, or -1.
+__device__ __forceinline__ int kv_page(const KvBatch &b, const KvCacheView &c, int s, int pos)
+{
+    const int i = kv_entry_of(pos, c.T, b.max_pages);
+    return i < 0 ? -1 : kv_page_of(b.pages[(size_t)s * b.max_pages + i], c.n_pages);
+}
+
+} // namespace dmoe

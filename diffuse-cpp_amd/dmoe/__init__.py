@@ -22,6 +22,7 @@ from ._abi import (AttnDesc, AttnHParams, Debug, HParams, LayerDesc, Tensor, TYP
                    TYPE_Q8_0, TYPE_Q8_K, TYPE_NAMES, TYPE_BY_NAME, row_size, block_elems,
                    block_bytes)
 from . import _abi
+from .kv import KvBatch, KvCache, attn_hparams
 
 PKG_DIR = Path(__file__).resolve().parent.parent
 LIB_PATH = PKG_DIR / "libdmoe.so"
@@ -37,7 +38,8 @@ EXPORTS = ("dmoe_create", "dmoe_destroy", "dmoe_last_error", "dmoe_layer_upload"
            "dmoe_gguf_moe_hparams", "dmoe_gguf_layer_desc", "dmoe_gguf_dense_desc",
            "dmoe_head_upload", "dmoe_head_wrap_device", "dmoe_head_forward", "dmoe_head_forward_device",
            "dmoe_attn_upload", "dmoe_attn_wrap_device", "dmoe_attn_forward", "dmoe_attn_forward_device",
-           "dmoe_gguf_attn_hparams", "dmoe_gguf_attn_desc")
+           "dmoe_gguf_attn_hparams", "dmoe_gguf_attn_desc", "dmoe_kv_append_device", "dmoe_kv_attn_device",
+           "dmoe_kv_attn_workspace", "dmoe_attn_forward_cached_device", "dmoe_attn_cached_workspace")
 NOALLOC_SCRATCH_BYTES = 64 << 20
 N_STAGES = 10
 PATH_NAMES = {0: "gemv", 1: "q4k_mfma", 2: "q80_mfma", 3: "f16_gemm", 4: "q6k_mfma", -1: "none"}
@@ -102,6 +104,13 @@ def load() -> C.CDLL:
     lib.dmoe_residual_rmsnorm.argtypes = [P, P, P, P, P, C.c_int32, C.c_int32, C.c_float, P]
     lib.dmoe_profile_enable.argtypes = [P, C.c_int]
     lib.dmoe_profile_read.argtypes = [P, P, P]
+    lib.dmoe_kv_append_device.argtypes = [P, P, P, C.POINTER(AttnHParams), P, P, P, P, P]
+    lib.dmoe_kv_attn_device.argtypes = [P, P, P, C.POINTER(AttnHParams), P, P, P, C.c_size_t, P]
+    lib.dmoe_kv_attn_workspace.argtypes = [P, P, P, C.POINTER(AttnHParams)]
+    lib.dmoe_kv_attn_workspace.restype = C.c_size_t
+    lib.dmoe_attn_forward_cached_device.argtypes = [P, P, P, P, P, P, P, P, C.c_size_t, P]
+    lib.dmoe_attn_cached_workspace.argtypes = [P, P, P, P]
+    lib.dmoe_attn_cached_workspace.restype = C.c_size_t
     lib.dmoe_stage_name.argtypes = [C.c_int]
     lib.dmoe_stage_name.restype = C.c_char_p
     _lib = lib
@@ -512,6 +521,47 @@ class Context:
                                                     _ptr(moe_in_dev) if moe_in_dev is not None else None,
                                                     s or None))
 
+    @staticmethod
+    def _ws(workspace):
+        return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+
+    def kv_append_device(self, cache: KvCache, batch: KvBatch, ap: AttnHParams, qkv, q_out, q_norm=None, k_norm=None,
+                         stream=None):
+        """Rows of the fused QKV projection into the paged cache, queries to
+        q_out (dmoe_kv_append_device)."""
+        self._check(load().dmoe_kv_append_device(
+            self.handle, cache.ref, batch.ref, ap, _ptr(qkv), None if q_norm is None else _ptr(q_norm),
+            None if k_norm is None else _ptr(k_norm), _ptr(q_out), stream or None))
+
+    def kv_attn_device(self, cache: KvCache, batch: KvBatch, ap: AttnHParams, q, out, workspace=None, stream=None):
+        """Attention of the batch's queries over the paged cache
+        (dmoe_kv_attn_device); workspace: a tensor of kv_attn_workspace bytes,
+        None for the context's own."""
+        ws, n = self._ws(workspace)
+        self._check(load().dmoe_kv_attn_device(self.handle, cache.ref, batch.ref, ap, _ptr(q), _ptr(out), ws, n,
+                                               stream or None))
+
+    def kv_attn_workspace(self, cache: KvCache, batch: KvBatch, ap: AttnHParams) -> int:
+        n = load().dmoe_kv_attn_workspace(self.handle, cache.ref, batch.ref, ap)
+        if not n:
+            raise DmoeError(_abi.ERR_INVALID_ARG, self.last_error())
+        return n
+
+    def attn_forward_cached_device(self, layer: Layer, cache: KvCache, batch: KvBatch, h_dev, h_out_dev,
+                                   moe_in_dev=None, workspace=None, stream=None):
+        """The attention half of a layer over a paged cache
+        (dmoe_attn_forward_cached_device)."""
+        ws, n = self._ws(workspace)
+        self._check(load().dmoe_attn_forward_cached_device(
+            self.handle, layer.handle, cache.ref, batch.ref, _ptr(h_dev), _ptr(h_out_dev),
+            None if moe_in_dev is None else _ptr(moe_in_dev), ws, n, stream or None))
+
+    def attn_cached_workspace(self, layer: Layer, cache: KvCache, batch: KvBatch) -> int:
+        n = load().dmoe_attn_cached_workspace(self.handle, layer.handle, cache.ref, batch.ref)
+        if not n:
+            raise DmoeError(_abi.ERR_INVALID_ARG, self.last_error())
+        return n
+
     def forward(self, layer: Layer, x: np.ndarray, debug: bool = False):
         x = np.ascontiguousarray(x, dtype=np.float32)
         N = x.shape[0]
@@ -576,5 +626,5 @@ class Context:
 
 
 __all__ = ["Context", "Layer", "LayerWeights", "DenseWeights", "HeadWeights", "AttnWeights", "DmoeError", "load", "tensor_view", "hparams_of",
-           "use_block_routing", "row_size", "TYPE_F32", "TYPE_F16", "TYPE_Q8_0", "TYPE_Q4_K",
+           "use_block_routing", "row_size", "KvCache", "KvBatch", "attn_hparams", "TYPE_F32", "TYPE_F16", "TYPE_Q8_0", "TYPE_Q4_K",
            "TYPE_Q8_K", "TYPE_NAMES", "TYPE_BY_NAME", "EXPORTS", "LIB_PATH"]

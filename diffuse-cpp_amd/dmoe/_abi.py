@@ -50,6 +50,17 @@ class AttnDesc(C.Structure):
     _fields_ = [(n, Tensor) for n in ("attn_norm", "qkv", "q_norm", "k_norm", "wo", "post_attn_norm")]
 
 
+class KvCacheStruct(C.Structure):
+    _fields_ = [("type", C.c_int32), ("n_head_kv", C.c_int32), ("head_dim", C.c_int32), ("page_tokens", C.c_int32),
+                ("n_pages", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p), ("k_exp", C.c_void_p),
+                ("v_exp", C.c_void_p)]
+
+
+class KvBatchStruct(C.Structure):
+    _fields_ = [("n_seqs", C.c_int32), ("n_tokens", C.c_int32), ("max_pages", C.c_int32), ("q_start", C.c_void_p),
+                ("kv_len", C.c_void_p), ("pages", C.c_void_p)]
+
+
 class Debug(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("probs", C.c_void_p), ("bmax", C.c_void_p),
                 ("thr", C.c_void_p), ("allowed", C.c_void_p), ("idx", C.c_void_p),

@@ -243,6 +243,114 @@ int  dmoe_attn_forward_device(dmoe_ctx *ctx, const dmoe_layer *attn, const float
                               int32_t n_tokens, float *h_out_dev, float *moe_in_dev,
                               void *stream);
 
+/* ---- a paged KV cache for the attention half ---------------------------
+ * The reference forms the keys and values of its whole window again in every
+ * step (src/diffuse-sampler.cpp:152-172), although the block-causal mask lets
+ * those of finished blocks change no more.  With a cache a step runs over the
+ * tokens of the current block only; with block_length 1 the same calls are
+ * those of a causal decoder.
+ *
+ * The cache is the caller's device memory, in pages of page_tokens (a multiple
+ * of 32) tokens, held per page, kv head and block of 32 tokens:
+ *   k  [n_pages][n_head_kv][page_tokens][head_dim]
+ *   v  [n_pages][n_head_kv][page_tokens / 32] blocks, transposed:
+ *      DMOE_KV_F16   [head_dim][32]
+ *      DMOE_KV_E4M3  [head_dim / 2][4][2][8]: token 8 b + j of dim 2 a + c at
+ *                    [a][b][c][j]
+ *   k_exp, v_exp  int8 [n_pages][n_head_kv][page_tokens / 32], DMOE_KV_E4M3
+ *      only: the values of a block are code * 2^exp, -50 <= exp <= 50
+ * F16 holds magnitudes up to 65504 (larger ones become infinite), E4M3 up to
+ * 448 * 2^50 (larger and infinite ones become NaN); an E4M3 block keeps four
+ * significant bits of every value within 2^14 of its largest one.  A page that
+ * has not been written may hold anything. */
+#define DMOE_KV_F16   0
+#define DMOE_KV_E4M3  1
+#define DMOE_KV_BLOCK 32
+typedef struct dmoe_kv_cache {
+    int32_t type;                /* DMOE_KV_F16 or DMOE_KV_E4M3               */
+    int32_t n_head_kv, head_dim; /* head_dim 64 or 128                        */
+    int32_t page_tokens;         /* a multiple of 32                          */
+    int32_t n_pages;
+    void   *k, *v;               /* 16-byte aligned                           */
+    int8_t *k_exp, *v_exp;       /* DMOE_KV_E4M3 only                         */
+} dmoe_kv_cache;
+
+/* The sequences of one call.  Their rows lie one after the other in the call's
+ * token buffers; a sequence without rows is allowed, and rows past the last
+ * sequence's are left as they are.  Token p of sequence s is in page
+ * pages[s * max_pages + p / page_tokens]; an entry outside 0 .. n_pages - 1
+ * (-1, say) and a token past the table hold nothing: an append skips them, the
+ * attention does not see them.  A sequence whose numbers contradict each other
+ * (rows outside 0 .. n_tokens, kv_len below its number of rows) is treated as
+ * one without rows.  The three tables are read on the stream: a captured call
+ * sees what they hold at each replay. */
+typedef struct dmoe_kv_batch {
+    int32_t n_seqs;
+    int32_t n_tokens;            /* rows of the token buffers                 */
+    int32_t max_pages;           /* entries of a sequence's row of `pages`    */
+    const int32_t *q_start;      /* [n_seqs + 1] device: first rows           */
+    const int32_t *kv_len;       /* [n_seqs] device: cached tokens, the rows of this call included */
+    const int32_t *pages;        /* [n_seqs][max_pages] device                */
+} dmoe_kv_batch;
+
+/* Rows of the fused QKV projection into the cache (the QK norm and rotation of
+ * src/diffuse-moe-graph.cpp:132-155): row i of sequence s is its token
+ * p = kv_len[s] - rows + i.  Query and key heads: RMSNorm over head_dim times
+ * q_norm_dev / k_norm_dev [head_dim] when ap->use_qk_norm, NEOX rotation of the
+ * first rotary_dim dims by p * rope_base^(-2 i / rotary_dim), in binary64 and
+ * rounded once (dmoe_attn_forward's angles follow ggml's chain of f32 products
+ * instead, which drifts with the position).  Queries go to
+ * q_out_dev [n_tokens][n_head][head_dim] f32, keys and values to the cache.
+ * Rows that a sequence holds at these positions already are replaced, which is
+ * how a denoising step writes its block again and how a cache is cut back.
+ * DMOE_KV_E4M3: rows that begin a block set its exponents anew, the least with
+ * amax <= 448 * 2^exp; rows that begin inside one keep the tokens before them,
+ * whose codes are rounded again where the exponent has to grow.  Two sequences
+ * of one call must not write into the same block of the same page.
+ * ap: n_embd, block_length are not used.  qkv_dev
+ * [n_tokens][(n_head + 2 n_head_kv) head_dim] f32 and q_out_dev do not overlap
+ * and are 16-byte aligned.  Queued on `stream` without synchronising; uses no
+ * workspace. */
+int  dmoe_kv_append_device(dmoe_ctx *ctx, const dmoe_kv_cache *kv, const dmoe_kv_batch *batch,
+                           const dmoe_attn_hparams *ap, const float *qkv_dev,
+                           const float *q_norm_dev, const float *k_norm_dev, float *q_out_dev,
+                           void *stream);
+
+/* Attention over the cache (src/diffuse-moe-graph.cpp:158-170): the query of
+ * token p of a sequence sees its cached tokens j with
+ * j / block_length <= p / block_length (all of them when block_length <= 0),
+ * scale 1 / sqrt(head_dim), query head h on kv head h / (n_head / n_head_kv);
+ * a query that sees nothing gives zeros, and what a query does not see has no
+ * part in its result whatever it holds.  q_dev, out_dev
+ * [n_tokens][n_head][head_dim] f32, 16-byte aligned, not overlapping; sums and
+ * softmax statistics in f32, at f32's accuracy on the cached values.
+ * ap: n_head, n_head_kv, head_dim and block_length are used.
+ * workspace_dev: dmoe_kv_attn_workspace bytes (16-byte aligned) that no other call in flight
+ * uses, or NULL for the context's own workspace, which grows on demand; a
+ * captured call brings its own.  Queued on `stream` without synchronising. */
+int  dmoe_kv_attn_device(dmoe_ctx *ctx, const dmoe_kv_cache *kv, const dmoe_kv_batch *batch,
+                         const dmoe_attn_hparams *ap, const float *q_dev, float *out_dev,
+                         void *workspace_dev, size_t workspace_bytes, void *stream);
+/* Bytes that call needs for these sizes (the tables are not read; pointers may
+ * be NULL); 0 for arguments that it refuses, with the reason in
+ * dmoe_last_error. */
+size_t dmoe_kv_attn_workspace(dmoe_ctx *ctx, const dmoe_kv_cache *kv, const dmoe_kv_batch *batch,
+                              const dmoe_attn_hparams *ap);
+
+/* dmoe_attn_forward_device over a cache: the rows h of the batch are normed
+ * and projected, their keys and values appended, and they attend to their own
+ * sequences' cached tokens; then the output projection, the residual and the
+ * post-attention norm.  Positions are the batch's.  h, h_out
+ * [n_tokens][n_embd] (h_out may be h); moe_in may be NULL; rows past the last
+ * sequence's get no attention and hold nothing of use.  Workspace as for
+ * dmoe_kv_attn_device, dmoe_attn_cached_workspace bytes. */
+int  dmoe_attn_forward_cached_device(dmoe_ctx *ctx, const dmoe_layer *attn, const dmoe_kv_cache *kv,
+                                     const dmoe_kv_batch *batch, const float *h_dev,
+                                     float *h_out_dev, float *moe_in_dev, void *workspace_dev,
+                                     size_t workspace_bytes, void *stream);
+size_t dmoe_attn_cached_workspace(dmoe_ctx *ctx, const dmoe_layer *attn, const dmoe_kv_cache *kv,
+                                  const dmoe_kv_batch *batch);
+
 /* Release a layer's device buffers.  The layer records its own device, so it
  * may be freed before or after the context that created it. */
 void dmoe_layer_free(dmoe_layer *layer);
