@@ -21,15 +21,18 @@ namespace dmoe {
 
 // Rows of a sequence in the call's token buffers and its cached tokens, these
 // rows included.  Entries that contradict each other (rows outside the buffers,
-// more rows than cached tokens) leave the sequence without rows, so that no
-// index derived from them leaves a buffer.
+// more rows than cached tokens, more tokens than KV_TOKENS_MOST) leave the
+// sequence without rows, so that no index derived from them leaves a buffer or
+// 32 bits.
 struct KvSeq {
     int q0, n, len;
 };
+constexpr int KV_TOKENS_MOST = 1 << 30;
 
 KV_HD KvSeq kv_seq_of(int start, int end, int len, int n_tokens)
 {
-    const bool ok = start >= 0 && end >= start && end <= n_tokens && len >= end - start;
+    const bool ok = start >= 0 && end >= start && end <= n_tokens && len >= end - start &&
+                    len <= KV_TOKENS_MOST;
     return KvSeq{start, ok ? end - start : 0, len};
 }
 

@@ -281,8 +281,8 @@ typedef struct dmoe_kv_cache {
  * pages[s * max_pages + p / page_tokens]; an entry outside 0 .. n_pages - 1
  * (-1, say) and a token past the table hold nothing: an append skips them, the
  * attention does not see them.  A sequence whose numbers contradict each other
- * (rows outside 0 .. n_tokens, kv_len below its number of rows) is treated as
- * one without rows.  The three tables are read on the stream: a captured call
+ * (rows outside 0 .. n_tokens, kv_len below its number of rows or above 2^30)
+ * is treated as one without rows.  The three tables are read on the stream: a captured call
  * sees what they hold at each replay. */
 typedef struct dmoe_kv_batch {
     int32_t n_seqs;

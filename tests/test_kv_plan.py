@@ -133,11 +133,12 @@ def test_refusals_of_null_structs_and_workspaces(ask):
 
 def test_sequences_of_any_table_stay_in_the_buffers(ask):
     big = 2 ** 31 - 1
-    edge = [-2 ** 31, -1, 0, 1, 31, 32, 33, 100, 101, big - 1, big]
+    most = 1 << 30
+    edge = [-2 ** 31, -1, 0, 1, 31, 32, 33, 100, 101, most, most + 1, big]
     calls = [("seq", [a, b, k, n]) for a, b, k in itertools.product(edge, edge, edge) for n in (1, 100)]
     for (_, (a, b, k, n)), r in zip(calls, ask(calls)):
         q0, rows, length, blocks = map(int, r.split())
-        ok = 0 <= a <= b <= n and k >= b - a
+        ok = 0 <= a <= b <= n and b - a <= k <= most
         assert rows == (b - a if ok else 0)
         if rows:
             assert 0 <= q0 and q0 + rows <= n and length - rows >= 0
