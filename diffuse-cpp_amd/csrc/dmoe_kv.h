@@ -18,6 +18,7 @@ namespace dmoe {
 
 typedef _Float16 kv_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 kv_h2 __attribute__((ext_vector_type(2)));
+typedef float kv_f2 __attribute__((ext_vector_type(2)));
 typedef float kv_f4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ KvSeq kv_seq(const KvBatch &b, int s)

@@ -18,6 +18,8 @@
 // probabilities (p' = 2^(s + ve - m'), at most 1 by the choice of m'), and the
 // sum takes p' 2^-ve: no operand is rescaled.  With exponents within 100 of
 // each other no p' that counts in the sum underflows.
+#include <type_traits>
+
 #include "dmoe_kv.h"
 
 #pragma clang fp contract(off)
@@ -25,9 +27,9 @@
 namespace dmoe {
 
 constexpr int KA_WAVES = 4;              // wavefronts of a workgroup
-constexpr int KA_COLS = 16;              // columns of an item
 constexpr int KA_SHIFT = 4;              // probabilities are held times 2^KA_SHIFT
 constexpr int KA_SLACK = 8;              // .. and may pass that by 2^KA_SLACK before their reference is raised
+constexpr int KA_COLS = 32;              // columns of an item at most
 constexpr int KA_CHUNK = 16;             // token tiles of a chunk at least
 constexpr int KA_ITEMS = 512;            // items wanted of a call
 
@@ -51,6 +53,15 @@ __device__ __forceinline__ void kv_widen(const uint4 &x, kv_h8 (&o)[F8 ? 2 : 1])
     }
 }
 
+// f16(p - hi), both halves: the difference is exact in f32
+__device__ __forceinline__ kv_h2 kv_rest(const kv_f2 &p, const kv_h2 &hi)
+{
+    kv_f2 r;
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r[0]) : "v"(hi), "v"(p[0]));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r[1]) : "v"(hi), "v"(p[1]));
+    return __builtin_convertvector(r, kv_h2);
+}
+
 // tokens 8 g .. 8 g + 7 of a block, those from `lim` on set to zero
 __device__ __forceinline__ kv_h8 kv_cut(const kv_h8 &v, int g, int lim)
 {
@@ -63,113 +74,183 @@ __device__ __forceinline__ kv_h8 kv_cut(const kv_h8 &v, int g, int lim)
 }
 
 // ---------------------------------------------------------------------------
-// Work items.  A sequence's columns form tiles of KA_COLS, its cached tokens
-// tiles of 32; an item is one column tile of one kv head over one chunk of
-// token tiles.  The chunk length is common to all sequences, so that ragged
-// ones spread over the chip like one: the total of (column tile, token tile)
-// pairs over the items wanted, at least KA_CHUNK.  A sequence's chunks are then
-// made equally long.
+// Work items.  A sequence's columns (query, head of a kv head) form tiles of 16
+// (up to 16 columns in all) or 32, its cached tokens tiles of 32; an item is
+// one column tile of one kv head over one chunk of token tiles.  The chunk
+// length is common to all sequences, so that ragged ones spread over the chip
+// like one: the total of (column tile, token tile) pairs over the items wanted,
+// at least KA_CHUNK.  A sequence's chunks are then made equally long.
+//
+// A sequence's items lie kv heads first, then chunks, then column tiles: what
+// reads the same keys is a multiple of the kv heads apart, and as workgroups go
+// to the 8 XCDs in turn, it shares few L2s (with 4 or 8 kv heads an XCD meets
+// two heads or one).
 struct KvItem {
-    int s, tile;                         // sequence, column tile
     KvSeq q;
+    int s, kvh, tile, split;             // sequence, kv head, column tile, chunk
+    int cb;                              // 16-column blocks of a tile
     int ks, chunk;                       // chunks of the sequence, token tiles of each
-    int split, first;                    // this item's chunk; the column tile's first item
 };
 
-__device__ __forceinline__ int kv_col_tiles(const KvSeq &q, int G) { return (int)(((int64_t)q.n * G + KA_COLS - 1) / KA_COLS); }
+// 16-column blocks of a tile of a sequence with `cols` columns
+__device__ __forceinline__ int kv_blocks_of_tile(int cols) { return cols <= 16 ? 1 : 2; }
 
 __device__ __forceinline__ int kv_token_tiles(const KvAttnArgs &a, const KvSeq &q)
 {
     return (kv_cached(q.len, a.c.T, a.b.max_pages) + 31) / 32;
 }
 
-// The common chunk length, by one wavefront.
-__device__ __forceinline__ int kv_chunk(const KvAttnArgs &a, int G)
+__device__ __forceinline__ int kv_col_tiles(const KvSeq &q, int G)
 {
-    const int lane = threadIdx.x & 63;
-    float w = 0.0f;                      // exact enough: a length, not an index
-    for (int base = 0; base < a.b.n_seqs; base += 64)
-        if (base + lane < a.b.n_seqs) {
-            const KvSeq q = kv_seq(a.b, base + lane);
-            w += (float)kv_col_tiles(q, G) * (float)kv_token_tiles(a, q);
-        }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) w += __shfl_xor(w, d, 64);
-    // rounded up beyond what the sum's rounding can hide
-    return max(KA_CHUNK, (int)(w / (float)a.items * 1.001f) + 1);
+    const int cols = q.n * G, per = 16 * kv_blocks_of_tile(cols);
+    return (cols + per - 1) / per;
 }
 
-// Item `item` of the call (units: column tiles, whatever their chunks), or
-// false past the last.
-__device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, bool units, KvItem &it)
+// Item `item` of the call, or false past the last.  One wavefront, 64
+// sequences at a time.
+__device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, KvItem &it)
 {
     const int lane = threadIdx.x & 63;
-    const int C = a.split ? kv_chunk(a, G) : 0x7fffffff;
-    int first = 0;
+    int C = 0x7fffffff;
+    if (a.split) {
+        float w = 0.0f;                  // exact enough: a length, not an index
+        for (int base = 0; base < a.b.n_seqs; base += 64)
+            if (base + lane < a.b.n_seqs) {
+                const KvSeq q = kv_seq(a.b, base + lane);
+                w += (float)kv_col_tiles(q, G) * (float)kv_token_tiles(a, q);
+            }
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) w += __shfl_xor(w, d, 64);
+        // rounded up beyond what the sum's rounding can hide
+        C = max(KA_CHUNK, (int)(w * (float)a.nkv / (float)KA_ITEMS * 1.001f) + 1);
+    }
     for (int base = 0; base < a.b.n_seqs; base += 64) {
         KvSeq q{0, 0, 0};
-        int nt = 0, ks = 0;
+        int tiles = 0, ks = 1;
         if (base + lane < a.b.n_seqs) {
             q = kv_seq(a.b, base + lane);
-            nt = kv_col_tiles(q, G);
+            tiles = kv_col_tiles(q, G);
             // (a sequence without tokens still has its rows to zero)
-            ks = max(1, a.split ? (kv_token_tiles(a, q) + C - 1) / C : 1);
+            if (a.split) ks = max(1, (kv_token_tiles(a, q) + C - 1) / C);
         }
-        const int mine = nt * ks, count = units ? nt : mine;
-        const int end = kv_wave_scan(count), items_end = units ? kv_wave_scan(mine) : end;
+        const int count = tiles * ks * a.nkv, end = kv_wave_scan(count);
         const uint64_t past = __ballot(end > item);
         if (past) {
             const int l = __builtin_ctzll(past);
             auto at = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
             it.s = base + l;
             it.q = KvSeq{at(q.q0), at(q.n), at(q.len)};
+            it.cb = kv_blocks_of_tile(it.q.n * G);
             it.ks = at(ks);
-            const int tiles = kv_token_tiles(a, it.q), i = item - (at(end) - at(count));
-            it.chunk = (tiles + it.ks - 1) / it.ks;
-            it.tile = units ? i : i / it.ks;
-            it.split = units ? 0 : i % it.ks;
-            it.first = first + at(items_end) - at(mine) + it.tile * it.ks;
+            it.chunk = (kv_token_tiles(a, it.q) + it.ks - 1) / it.ks;
+            const int i = item - (at(end) - at(count));
+            it.kvh = i % a.nkv;
+            it.split = i / a.nkv % it.ks;
+            it.tile = i / a.nkv / it.ks;
             return true;
         }
         item -= __builtin_amdgcn_readlane(end, 63);
-        first += __builtin_amdgcn_readlane(items_end, 63);
     }
     return false;
 }
 
-// Partial results of an item in the workspace: its columns' sums [KA_COLS][HD],
-// then their (m, l).
+// The workspace of a call whose sequences can have several chunks: per item
+// what the join has to know, then its columns' sums [KA_COLS][HD] and
+// their (m, l).
+struct KvDesc {
+    int32_t ks, tile, kvh, q0, cols, cb;         // ks 0: no chunk, or not the first of several
+    int32_t pad[2];
+};
+
 template <int HD>
-__device__ __forceinline__ float *kv_part(const KvAttnArgs &a, int item, int kvh)
+__device__ __forceinline__ float *kv_part(const KvAttnArgs &a, int item)
 {
-    return (float *)a.ws + ((size_t)item * a.nkv + kvh) * KA_COLS * (HD + 2);
+    return (float *)((KvDesc *)a.ws + a.items) + (size_t)item * KA_COLS * (HD + 2);
 }
 
-template <int HD, bool F8>
-__global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn(KvAttnArgs a)
+// One item's columns, 16 CB of them: the workgroup's wavefronts take its token
+// tiles in turn and join their results in LDS.  A tile's keys and values go
+// straight from global memory to the registers that hold them as operands; the
+// next tile's keys are loaded once a tile's scores stand, its values once its
+// sums do, so that loads are always in flight and no second set of registers
+// is needed.
+template <int HD, bool F8, int CB>
+__device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it, int G, float *s_o, float *s_m, float *s_l)
 {
     constexpr int NC = HD / 32;                    // 32-dim chunks of a row
     constexpr int NB = HD / 16;                    // 16-dim blocks of O
-    constexpr int EB = F8 ? 1 : 2;
+    constexpr int EB = F8 ? 1 : 2, NE = F8 ? 2 : 1;
     constexpr int NK = HD * EB / 32;               // 16-byte pieces a lane loads of a tile's keys, and of its values
     constexpr int LO = HD + 4;                     // row of O in LDS: padded against bank conflicts
-    __shared__ __align__(16) float s_o[KA_WAVES][KA_COLS * LO];
-    __shared__ float s_m[KA_WAVES][KA_COLS], s_l[KA_WAVES][KA_COLS];
     const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int G = a.nh / a.nkv, kvh = blockIdx.x % a.nkv;
-    KvItem it;
-    if (!kv_item(a, G, blockIdx.x / a.nkv, false, it)) return;
     const KvSeq q = it.q;
-    // this lane's column: query q.q0 + qi, head kvh G + hg
-    const int col = it.tile * KA_COLS + r16;
-    const bool live = col < q.n * G;
-    const int qi = live ? col / G : 0, hg = live ? col % G : 0;
-    const size_t at = ((size_t)(q.q0 + qi) * a.nh + (size_t)kvh * G + hg) * HD;
-    // tokens the column sees: 0 .. vis - 1
+    const int kvh = it.kvh;
     const int cached = kv_cached(q.len, a.c.T, a.b.max_pages);
-    const int vis = live ? kv_visible(q.len - q.n + qi, cached, a.block) : 0;
-    int last = vis, least = live ? vis : cached;
+    const float inf = __builtin_inff(), low = -3.402823466e38f;
+
+    // this lane's columns: query q.q0 + col / G, head kvh G + col % G; tokens
+    // 0 .. vis - 1 are what it sees
+    int vis[CB], last = 0, least = cached;
+#pragma unroll
+    for (int cb = 0; cb < CB; cb++) {
+        const int col = (it.tile * CB + cb) * 16 + r16;
+        const bool live = col < q.n * G;
+        vis[cb] = live ? kv_visible(q.len - q.n + col / G, cached, a.block) : 0;
+        last = max(last, vis[cb]);
+        if (live) least = min(least, vis[cb]);
+    }
+    // the queries as operands in LDS, [16-column block][chunk][hi, lo][lane]:
+    // every wavefront has the same, and registers are short.  Chunk 2 p + e of a
+    // lane holds dims 64 p + 16 g + 8 e .. + 7 (its 16 dims of a 64-dim half are
+    // one piece of an E4M3 key row)
+    kv_h8 *s_q = reinterpret_cast<kv_h8 *>(s_o);
+    if (w < CB) {
+        const int col = (it.tile * CB + w) * 16 + r16;
+        const bool live = col < q.n * G;
+        const int qi = live ? col / G : 0, hg = live ? col % G : 0;
+        const float *src = a.q + ((size_t)(q.q0 + qi) * a.nh + (size_t)kvh * G + hg) * HD + 16 * g;
+        float x[NC][8], amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(src + 64 * (c / 2) + 8 * (c % 2) + j);
+                x[c][j] = v.x;
+                x[c][j + 1] = v.y;
+                x[c][j + 2] = v.z;
+                x[c][j + 3] = v.w;
+            }
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[c][j] = live ? x[c][j] : 0.0f;
+                amax = fmaxf(amax, fabsf(x[c][j]));
+            }
+        amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+        int up = 0;
+        if (amax > 0.0f && amax <= 3.402823466e38f) {
+            int ex;
+            (void)frexpf(amax, &ex);
+            up = min(8 - ex, 100);
+        }
+        const float mul = ldexpf(1.0f, up);
+        if (g == 0) s_m[16 * w + r16] = ldexpf(a.scale * 1.44269504088896341f, -up);
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            kv_h8 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float y = x[c][j] * mul;
+                hi[j] = (_Float16)y;
+                lo[j] = (_Float16)(y - (float)hi[j]);
+            }
+            s_q[((w * NC + c) * 2 + 0) * 64 + lane] = hi;
+            s_q[((w * NC + c) * 2 + 1) * 64 + lane] = lo;
+        }
+    }
 #pragma unroll
     for (int d = 8; d >= 1; d >>= 1) {
         last = max(last, __shfl_xor(last, d, 64));
@@ -180,322 +261,374 @@ __global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn(KvAttnArgs a)
     // this wavefront's token tiles: tile0 + w, every KA_WAVES-th, up to tile1
     const int tile0 = it.split * it.chunk, tile1 = min(tile0 + it.chunk, (last + 31) / 32);
 
-    // queries: chunk 2 p + e of this lane holds dims 64 p + 16 g + 8 e .. + 7
-    // (a lane's 16 dims of a 64-dim half are one piece of an E4M3 key row)
-    kv_h8 qh[NC], ql[NC];
-    float cmul;
-    {
-        float x[NC][8], amax = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; c++) {
-            const float *src = a.q + at + 64 * (c / 2) + 16 * g + 8 * (c % 2);
-#pragma unroll
-            for (int j = 0; j < 8; j += 4) {
-                const float4 v = live ? *reinterpret_cast<const float4 *>(src + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-                x[c][j] = v.x;
-                x[c][j + 1] = v.y;
-                x[c][j + 2] = v.z;
-                x[c][j + 3] = v.w;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(x[c][j]));
-        }
-        amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-        int up = 0;
-        if (amax > 0.0f && amax <= 3.402823466e38f) {
-            int ex;
-            (void)frexpf(amax, &ex);
-            up = min(8 - ex, 100);
-        }
-        const float mul = ldexpf(1.0f, up);
-        cmul = ldexpf(a.scale * 1.44269504088896341f, -up);
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float y = x[c][j] * mul;
-                qh[c][j] = (_Float16)y;
-                ql[c][j] = (_Float16)(y - (float)qh[c][j]);
-            }
-    }
-
     // m: the columns' reference of s + ve, raised when a score passes it by
     // KA_SLACK (-inf: nothing seen; at least -FLT_MAX else, so that a row whose
     // every score is -inf ends as 0 / 0, not as empty); l: this lane's share of
     // the sum
-    const float inf = __builtin_inff(), low = -3.402823466e38f;
-    float m = -inf, l = 0.0f;
-    kv_f4 o[NB];
+    float m[CB], l[CB];
+    kv_f4 o[CB][NB];
 #pragma unroll
-    for (int b = 0; b < NB; b++) o[b] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int cb = 0; cb < CB; cb++) {
+        m[cb] = -inf;
+        l[cb] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; b++) o[cb][b] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
-    struct Tile {
-        uint4 k[NK], v[NK];
-    };
     // row r of key block kb is token 8 (r / 4) + 4 kb + r % 4, so that the
     // scores of a lane are those of tokens 8 g + 4 kb + i
     const uint32_t koff = (8 * (r16 >> 2) + (r16 & 3)) * HD * EB + 16 * EB * g;
     const uint32_t voff = (r16 * 4 + g) * 16;
-    auto load = [&](Tile &x, size_t byte) {
-        const uint8_t *K = (const uint8_t *)a.c.k + byte, *V = (const uint8_t *)a.c.v + byte;
+    uint4 kr[NK], vr[NK];
+    auto load_k = [&](size_t byte) {
+        const uint8_t *K = (const uint8_t *)a.c.k + byte;
 #pragma unroll
         for (int i = 0; i < NK; i++) {
             // key block, then chunk (F16) or pair of chunks (E4M3)
-            const int kb = i / (NK / 2), ch = i % (NK / 2) * (F8 ? 2 : 1);
-            x.k[i] = *reinterpret_cast<const uint4 *>(K + koff + 4 * kb * HD * EB + (64 * (ch / 2) + 8 * (ch % 2)) * EB);
-        }
-#pragma unroll
-        for (int i = 0; i < NK; i++) x.v[i] = *reinterpret_cast<const uint4 *>(V + voff + 1024 * i);
-    };
-    auto compute = [&](const Tile &x, int k0, int ke, int ve) {
-        const float c = F8 ? ldexpf(cmul, ke) : cmul, back = F8 ? ldexpf(1.0f, -ve) : 1.0f;
-        kv_f4 sc[2];
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++) {
-            sc[kb] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int ch = 0; ch < NC; ch += F8 ? 2 : 1) {
-                kv_h8 kf[F8 ? 2 : 1];
-                kv_widen<F8>(x.k[kb * (NK / 2) + ch / (F8 ? 2 : 1)], kf);
-#pragma unroll
-                for (int e = 0; e < (F8 ? 2 : 1); e++) {
-                    sc[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[e], ql[ch + e], sc[kb], 0, 0, 0);
-                    sc[kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[e], qh[ch + e], sc[kb], 0, 0, 0);
-                }
-            }
-        }
-        const bool whole = k0 + 32 <= least;       // every column sees the tile
-        float smax = -inf;
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                smax = fmaxf(smax, whole || k0 + 8 * g + 4 * kb + i < vis ? sc[kb][i] : -inf);
-        float mt = __builtin_fmaf(smax, c, (float)ve);
-        mt = vis > k0 ? fmaxf(mt, low) : -inf;
-        if (__any(mt > m + (float)KA_SLACK)) {
-            mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-            const float mn = fmaxf(m, mt);
-            const float corr = m == -inf ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= corr;
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[b][i] *= corr;
-        }
-        const float k = (float)ve + (float)KA_SHIFT - (m == -inf ? 0.0f : m);
-        float sum = 0.0f;
-        kv_h8 ph, pl;
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[kb][i], c, k));
-                p = whole || k0 + 8 * g + 4 * kb + i < vis ? p : 0.0f;
-                sum += p;
-                ph[4 * kb + i] = (_Float16)p;
-                pl[4 * kb + i] = (_Float16)(p - (float)ph[4 * kb + i]);
-            }
-        l = __builtin_fmaf(sum, back, l);
-        // values: O rows are dims 16 b + row (F16), 32 (b / 2) + 2 row + b % 2 (E4M3)
-        kv_h8 vf[NB];
-#pragma unroll
-        for (int i = 0; i < NK; i++) {
-            kv_h8 y[F8 ? 2 : 1];
-            kv_widen<F8>(x.v[i], y);
-#pragma unroll
-            for (int e = 0; e < (F8 ? 2 : 1); e++) vf[i * (F8 ? 2 : 1) + e] = y[e];
-        }
-        if (whole) {
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[b], pl, o[b], 0, 0, 0);
-                o[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[b], ph, o[b], 0, 0, 0);
-            }
-            return;
-        }
-        // some column does not see all 32 tokens: what it does not see may hold
-        // anything (0 times a NaN is one), so the columns of each limit in turn
-        // add a product whose values end there
-        for (int done = k0;;) {
-            int lim = vis > done ? vis : 0x7fffffff;
-#pragma unroll
-            for (int d = 8; d >= 1; d >>= 1) lim = min(lim, __shfl_xor(lim, d, 64));
-            lim = __builtin_amdgcn_readfirstlane(lim);
-            if (lim == 0x7fffffff) break;
-            const bool mine = vis > done && (vis == lim || lim >= k0 + 32);
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const kv_h8 y = kv_cut(vf[b], g, lim - k0);
-                kv_f4 t = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
-                t = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl, t, 0, 0, 0);
-                t = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ph, t, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[b][i] += mine ? t[i] : 0.0f;
-            }
-            if (lim >= k0 + 32) break;
-            done = lim;
+            const int kb = i / (NK / 2), ch = i % (NK / 2) * NE;
+            kr[i] = *reinterpret_cast<const uint4 *>(K + koff + 4 * kb * HD * EB + (64 * (ch / 2) + 8 * (ch % 2)) * EB);
         }
     };
+    auto load_v = [&](size_t byte) {
+        const uint8_t *V = (const uint8_t *)a.c.v + byte;
+#pragma unroll
+        for (int i = 0; i < NK; i++) vr[i] = *reinterpret_cast<const uint4 *>(V + voff + 1024 * i);
+    };
+
+    __syncthreads();
+    float cmul[CB];
+#pragma unroll
+    for (int cb = 0; cb < CB; cb++) cmul[cb] = s_m[16 * cb + r16];
 
     // up to 64 of the wavefront's tiles at a time: a lane looks up one tile's
     // page and exponents, and the loop takes them from there
     for (int base = tile0 + w; base < tile1; base += 64 * KA_WAVES) {
-        const int t = base + KA_WAVES * lane, k0 = 32 * t;
-        int page = -1, ke = 0, ve = 0;
-        if (t < tile1) page = kv_page(a.b, a.c, it.s, k0);
-        const size_t slot = ((size_t)max(page, 0) * a.nkv + kvh) * (a.c.T / 32) + k0 % a.c.T / 32;
+        const int tt = base + KA_WAVES * lane;
+        int page = -1, kes = 0, ves = 0;
+        if (tt < tile1) page = kv_page(a.b, a.c, it.s, 32 * tt);
+        const size_t slot = ((size_t)max(page, 0) * a.nkv + kvh) * (a.c.T / 32) + tt % (a.c.T / 32);
         if (F8 && page >= 0) {
-            ke = a.c.k_exp[slot];
-            ve = a.c.v_exp[slot];
+            kes = a.c.k_exp[slot];
+            ves = a.c.v_exp[slot];
         }
-        const size_t byte = slot * 32 * HD * EB;
-        const uint32_t blo = (uint32_t)byte, bhi = (uint32_t)(byte >> 32);
+        const uint32_t blo = (uint32_t)(slot * 32 * HD * EB), bhi = (uint32_t)(slot * 32 * HD * EB >> 32);
         auto where = [&](int i) {
             return (size_t)(uint32_t)__builtin_amdgcn_readlane(bhi, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(blo, i);
         };
         uint64_t todo = __ballot(page >= 0);
         if (!todo) continue;
-        // the next tile's loads are in flight during a tile's products (past
-        // the last one, that tile again: a wait counts loads, so there must
-        // always be some)
-        Tile x, y;
         int i = __builtin_ctzll(todo);
-        todo &= todo - 1;
-        load(x, where(i));
-        auto step = [&](Tile &now, Tile &next) {
-            const int j = todo ? __builtin_ctzll(todo) : i;
-            load(next, where(j));
-            compute(now, 32 * (base + KA_WAVES * i), __builtin_amdgcn_readlane(ke, i), __builtin_amdgcn_readlane(ve, i));
-            const bool more = todo != 0;
+        load_k(where(i));
+        load_v(where(i));
+        // tiles while `more` of them; FULL: every column sees all of each.  The
+        // references are raised outside the loop over tiles (the tile's scores
+        // are then formed again): a conditional change of the sums inside it
+        // costs a copy of them all per tile.
+        auto run = [&](auto full, auto &&more) {
+          constexpr bool FULL = decltype(full)::value;
+          for (;;) {
+            bool raise = false;
+            float mt[CB];
+            while (more()) {
+            const int k0 = 32 * (base + KA_WAVES * i), ve = F8 ? __builtin_amdgcn_readlane(ves, i) : 0;
+            const int ke = F8 ? __builtin_amdgcn_readlane(kes, i) : 0;
+            int ql0 = lane;
+            asm volatile("" : "+v"(ql0));          // the queries are read again each tile, not kept in registers
+            kv_f4 sc[CB][2];
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++)
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++) sc[cb][kb] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ch = 0; ch < NC; ch += NE) {
+                kv_h8 kf[2][NE];
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++) kv_widen<F8>(kr[kb * (NK / 2) + ch / NE], kf[kb]);
+#pragma unroll
+                for (int e = 0; e < NE; e++)
+#pragma unroll
+                    for (int cb = 0; cb < CB; cb++) {
+                        const kv_h8 qh = s_q[((cb * NC + ch + e) * 2 + 0) * 64 + ql0];
+                        const kv_h8 ql = s_q[((cb * NC + ch + e) * 2 + 1) * 64 + ql0];
+#pragma unroll
+                        for (int kb = 0; kb < 2; kb++) {
+                            sc[cb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kb][e], ql, sc[cb][kb], 0, 0, 0);
+                            sc[cb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kb][e], qh, sc[cb][kb], 0, 0, 0);
+                        }
+                    }
+            }
+            auto seen = [&](int cb, int kb, int e) { return FULL || k0 + 8 * g + 4 * kb + e < vis[cb]; };
+            float c[CB];
+            bool above = false;
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++) {
+                c[cb] = F8 ? ldexpf(cmul[cb], ke) : cmul[cb];
+                float smax = -inf;
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) smax = fmaxf(smax, seen(cb, kb, e) ? sc[cb][kb][e] : -inf);
+                mt[cb] = fmaxf(__builtin_fmaf(smax, c[cb], (float)ve), low);
+                if (!FULL) mt[cb] = vis[cb] > k0 ? mt[cb] : -inf;
+                above |= mt[cb] > m[cb] + (float)KA_SLACK;
+            }
+            if (__any(above)) {
+                raise = true;
+                break;
+            }
             todo &= todo - 1;
-            i = j;
-            return more;
+            // (past the last tile it is loaded again: a wait counts loads, so
+            // there must always be some)
+            if (todo) i = __builtin_ctzll(todo);
+            const size_t next = where(i);
+            load_k(next);
+            kv_h8 ph[CB], pl[CB];
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++) {
+                const float k = (float)(ve + KA_SHIFT) - (!FULL && m[cb] == -inf ? 0.0f : m[cb]);
+                float sum = 0.0f;
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        kv_f2 p;
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cb][kb][e + x], c[cb], k));
+                            p[x] = seen(cb, kb, e + x) ? p[x] : 0.0f;
+                            sum += p[x];
+                        }
+                        const kv_h2 hi = __builtin_convertvector(p, kv_h2), lo = kv_rest(p, hi);
+                        ph[cb][4 * kb + e] = hi[0];
+                        ph[cb][4 * kb + e + 1] = hi[1];
+                        pl[cb][4 * kb + e] = lo[0];
+                        pl[cb][4 * kb + e + 1] = lo[1];
+                    }
+                l[cb] = F8 ? __builtin_fmaf(sum, ldexpf(1.0f, -ve), l[cb]) : l[cb] + sum;
+            }
+            // values: O rows are dims 16 b + row (F16), 32 (b / 2) + 2 row + b % 2 (E4M3)
+            if (FULL) {
+#pragma unroll
+                for (int p = 0; p < NK; p++) {
+                    kv_h8 vf[NE];
+                    kv_widen<F8>(vr[p], vf);
+#pragma unroll
+                    for (int e = 0; e < NE; e++)
+#pragma unroll
+                        for (int cb = 0; cb < CB; cb++) {
+                            const int b = p * NE + e;
+                            o[cb][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[e], pl[cb], o[cb][b], 0, 0, 0);
+                            o[cb][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[e], ph[cb], o[cb][b], 0, 0, 0);
+                        }
+                }
+            } else {
+                // what a column does not see may hold anything (0 times a NaN
+                // is one), so the columns of each limit in turn add a product
+                // whose values end there
+                for (int done = k0;;) {
+                    int lim = 0x7fffffff;
+#pragma unroll
+                    for (int cb = 0; cb < CB; cb++)
+                        if (vis[cb] > done) lim = min(lim, vis[cb]);
+#pragma unroll
+                    for (int d = 8; d >= 1; d >>= 1) lim = min(lim, __shfl_xor(lim, d, 64));
+                    lim = __builtin_amdgcn_readfirstlane(lim);
+                    if (lim == 0x7fffffff) break;
+#pragma unroll
+                    for (int p = 0; p < NK; p++) {
+                        kv_h8 vf[NE];
+                        kv_widen<F8>(vr[p], vf);
+#pragma unroll
+                        for (int e = 0; e < NE; e++) {
+                            const kv_h8 y = kv_cut(vf[e], g, lim - k0);
+#pragma unroll
+                            for (int cb = 0; cb < CB; cb++) {
+                                const bool mine = vis[cb] > done && (vis[cb] == lim || lim >= k0 + 32);
+                                kv_f4 t = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                                t = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl[cb], t, 0, 0, 0);
+                                t = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ph[cb], t, 0, 0, 0);
+#pragma unroll
+                                for (int x = 0; x < 4; x++) o[cb][p * NE + e][x] += mine ? t[x] : 0.0f;
+                            }
+                        }
+                        __builtin_amdgcn_sched_barrier(0);     // one piece at a time: registers are short
+                    }
+                    if (lim >= k0 + 32) break;
+                    done = lim;
+                }
+            }
+            load_v(next);
+            }
+            if (!raise) break;
+#pragma unroll
+            for (int cb = 0; cb < CB; cb++) {
+                mt[cb] = fmaxf(mt[cb], __shfl_xor(mt[cb], 16, 64));
+                mt[cb] = fmaxf(mt[cb], __shfl_xor(mt[cb], 32, 64));
+                const float mn = fmaxf(m[cb], mt[cb]);
+                const float corr = m[cb] == -inf ? 0.0f : __builtin_amdgcn_exp2f(m[cb] - mn);
+                m[cb] = mn;
+                l[cb] *= corr;
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[cb][b][e] *= corr;
+            }
+          }
         };
-        while (step(x, y) && step(y, x)) {
-        }
+        run(std::true_type{}, [&] { return todo && 32 * (base + KA_WAVES * i) + 32 <= least; });
+        run(std::false_type{}, [&] { return todo != 0; });
     }
 
-    // the wavefronts' results joined in LDS
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    // the wavefronts' results joined in LDS: [wavefront][column][dim]
+    __syncthreads();                               // the queries' place, no longer needed
 #pragma unroll
-    for (int b = 0; b < NB; b += F8 ? 2 : 1)
-        if constexpr (F8) {
+    for (int cb = 0; cb < CB; cb++) {
+        l[cb] += __shfl_xor(l[cb], 16, 64);
+        l[cb] += __shfl_xor(l[cb], 32, 64);
+        float *dst = s_o + ((w * CB + cb) * 16 + r16) * LO;
 #pragma unroll
-            for (int i = 0; i < 4; i += 2)
-                *reinterpret_cast<float4 *>(&s_o[w][r16 * LO + 16 * b + 8 * g + 2 * i]) =
-                    make_float4(o[b][i], o[b + 1][i], o[b][i + 1], o[b + 1][i + 1]);
-        } else {
-            *reinterpret_cast<float4 *>(&s_o[w][r16 * LO + 16 * b + 4 * g]) = make_float4(o[b][0], o[b][1], o[b][2], o[b][3]);
+        for (int b = 0; b < NB; b += NE)
+            if constexpr (F8) {
+#pragma unroll
+                for (int i = 0; i < 4; i += 2)
+                    *reinterpret_cast<float4 *>(dst + 16 * b + 8 * g + 2 * i) =
+                        make_float4(o[cb][b][i], o[cb][b + 1][i], o[cb][b][i + 1], o[cb][b + 1][i + 1]);
+            } else {
+                *reinterpret_cast<float4 *>(dst + 16 * b + 4 * g) = make_float4(o[cb][b][0], o[cb][b][1], o[cb][b][2], o[cb][b][3]);
+            }
+        if (g == 0) {
+            s_m[(w * CB + cb) * 16 + r16] = m[cb];
+            s_l[(w * CB + cb) * 16 + r16] = l[cb];
         }
-    if (g == 0) {
-        s_m[w][r16] = m;
-        s_l[w][r16] = l;
     }
     __syncthreads();
-    const int cols = min(KA_COLS, q.n * G - it.tile * KA_COLS);
+    constexpr int COLS = 16 * CB;
+    const int cols = min(COLS, q.n * G - it.tile * COLS);
     for (int e = threadIdx.x; e < cols * (HD / 4); e += KA_WAVES * 64) {
         const int c = e / (HD / 4), d = e % (HD / 4) * 4;
-        float M = s_m[0][c];
+        float M = s_m[c];
 #pragma unroll
-        for (int i = 1; i < KA_WAVES; i++) M = fmaxf(M, s_m[i][c]);
+        for (int i = 1; i < KA_WAVES; i++) M = fmaxf(M, s_m[i * COLS + c]);
         float L = 0.0f;
         float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int i = 0; i < KA_WAVES; i++) {
-            const float f = s_m[i][c] == -inf ? 0.0f : __builtin_amdgcn_exp2f(s_m[i][c] - M);
-            const float4 x = *reinterpret_cast<const float4 *>(&s_o[i][c * LO + d]);
-            L += s_l[i][c] * f;
+            const float mi = s_m[i * COLS + c], f = mi == -inf ? 0.0f : __builtin_amdgcn_exp2f(mi - M);
+            const float4 x = *reinterpret_cast<const float4 *>(&s_o[(i * COLS + c) * LO + d]);
+            L += s_l[i * COLS + c] * f;
             O.x += x.x * f;
             O.y += x.y * f;
             O.z += x.z * f;
             O.w += x.w * f;
         }
         if (it.ks == 1) {
-            const int cc = it.tile * KA_COLS + c;
+            const int cc = it.tile * COLS + c;
             const float inv = M == -inf ? 0.0f : 1.0f / L;         // nothing seen: zeros
             *reinterpret_cast<float4 *>(a.out + ((size_t)(q.q0 + cc / G) * a.nh + (size_t)kvh * G + cc % G) * HD + d) =
                 make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
         } else {
-            float *part = kv_part<HD>(a, it.first + it.split, kvh);
+            float *part = kv_part<HD>(a, blockIdx.x);
             *reinterpret_cast<float4 *>(part + c * HD + d) = O;
             if (d == 0) *reinterpret_cast<float2 *>(part + KA_COLS * HD + 2 * c) = make_float2(M, L);
         }
     }
 }
 
-// Joins the chunks of a column: a workgroup takes one column, its wavefronts
-// every KA_WAVES-th chunk.
-template <int HD>
-__global__ __launch_bounds__(KA_WAVES * 64) void k_kv_join(KvAttnArgs a)
+template <int HD, bool F8>
+__global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn(KvAttnArgs a)
 {
-    constexpr int ND = HD / 64;                    // dims of a lane
-    __shared__ float s_o[KA_WAVES][HD], s_l[KA_WAVES];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int G = a.nh / a.nkv, kvh = blockIdx.y % a.nkv, c = blockIdx.y / a.nkv;
+    __shared__ __align__(16) float s_o[KA_WAVES * KA_COLS * (HD + 4)];
+    __shared__ float s_m[KA_WAVES * KA_COLS], s_l[KA_WAVES * KA_COLS];
+    const int G = a.nh / a.nkv;
     KvItem it;
-    if (!kv_item(a, G, blockIdx.x, true, it) || it.ks == 1) return;
-    const int col = it.tile * KA_COLS + c;
-    if (col >= it.q.n * G) return;
-    const float inf = __builtin_inff();
-    // the chunks' references: every lane those of chunks lane, lane + 64, ..
-    float M = -inf;
-    for (int j = lane; j < it.ks; j += 64) M = fmaxf(M, kv_part<HD>(a, it.first + j, kvh)[KA_COLS * HD + 2 * c]);
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
-    float o[ND] = {}, l = 0.0f;
-#pragma unroll 8
-    for (int j = w; j < it.ks; j += KA_WAVES) {
-        const float *part = kv_part<HD>(a, it.first + j, kvh);
-        const float2 ml = *reinterpret_cast<const float2 *>(part + KA_COLS * HD + 2 * c);
-        const float f = ml.x == -inf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
-        l += ml.y * f;
-#pragma unroll
-        for (int d = 0; d < ND; d++) o[d] += part[c * HD + ND * lane + d] * f;
+    const bool some = kv_item(a, G, blockIdx.x, it);
+    if (a.split && threadIdx.x == 0) {
+        KvDesc d{};
+        if (some && it.split == 0 && it.ks > 1)
+            d = KvDesc{it.ks, it.tile, it.kvh, it.q.q0, min(16 * it.cb, it.q.n * G - it.tile * 16 * it.cb), it.cb, {}};
+        ((KvDesc *)a.ws)[blockIdx.x] = d;
     }
-#pragma unroll
-    for (int d = 0; d < ND; d++) s_o[w][ND * lane + d] = o[d];
-    if (lane == 0) s_l[w] = l;
-    __syncthreads();
-    if (threadIdx.x >= HD) return;
-    float O = 0.0f, L = 0.0f;
-#pragma unroll
-    for (int i = 0; i < KA_WAVES; i++) {
-        O += s_o[i][threadIdx.x];
-        L += s_l[i];
-    }
-    a.out[((size_t)(it.q.q0 + col / G) * a.nh + (size_t)kvh * G + col % G) * HD + threadIdx.x] = M == -inf ? 0.0f : O / L;
+    if (!some) return;
+    if (it.cb == 1)
+        kv_attend<HD, F8, 1>(a, it, G, s_o, s_m, s_l);
+    else
+        kv_attend<HD, F8, 2>(a, it, G, s_o, s_m, s_l);
 }
 
-// What the launches take: the items wanted per kv head and at most, and whether
-// any sequence can have several chunks (from the page table's width: the
-// lengths themselves are on the GPU).
+// Joins the chunks of a column tile: a workgroup takes KJ_COLS of its columns,
+// its threads four dims of a column and every KJ_PARTS-th chunk.
+constexpr int KJ_COLS = 2;
+template <int HD>
+__global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a)
+{
+    constexpr int ND = HD / 4, PARTS = 256 / (KJ_COLS * ND);
+    __shared__ __align__(16) float4 s_o[PARTS][KJ_COLS][ND];
+    __shared__ float s_m[PARTS][KJ_COLS], s_l[PARTS][KJ_COLS];
+    const KvDesc d = ((const KvDesc *)a.ws)[blockIdx.x];
+    const int c0 = blockIdx.y * KJ_COLS;
+    if (d.ks == 0 || c0 >= d.cols) return;
+    const int e = threadIdx.x % ND, ci = threadIdx.x / ND % KJ_COLS, part = threadIdx.x / (ND * KJ_COLS);
+    const int c = min(c0 + ci, d.cols - 1);
+    const float inf = __builtin_inff();
+    float m = -inf, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int j = part; j < d.ks; j += PARTS) {
+        const float *p = kv_part<HD>(a, blockIdx.x + j * a.nkv);
+        const float2 ml = *reinterpret_cast<const float2 *>(p + KA_COLS * HD + 2 * c);
+        const float4 x = *reinterpret_cast<const float4 *>(p + c * HD + 4 * e);
+        const float mn = fmaxf(m, ml.x);
+        const float f = m == -inf ? 0.0f : __builtin_amdgcn_exp2f(m - mn), h = ml.x == -inf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+        m = mn;
+        l = l * f + ml.y * h;
+        o = make_float4(o.x * f + x.x * h, o.y * f + x.y * h, o.z * f + x.z * h, o.w * f + x.w * h);
+    }
+    s_o[part][ci][e] = o;
+    if (e == 0) {
+        s_m[part][ci] = m;
+        s_l[part][ci] = l;
+    }
+    __syncthreads();
+    if (part > 0 || c0 + ci >= d.cols) return;
+#pragma unroll
+    for (int i = 1; i < PARTS; i++) m = fmaxf(m, s_m[i][ci]);
+    l = 0.0f;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < PARTS; i++) {
+        const float f = s_m[i][ci] == -inf ? 0.0f : __builtin_amdgcn_exp2f(s_m[i][ci] - m);
+        const float4 x = s_o[i][ci][e];
+        l += s_l[i][ci] * f;
+        o = make_float4(o.x + x.x * f, o.y + x.y * f, o.z + x.z * f, o.w + x.w * f);
+    }
+    const int G = a.nh / a.nkv, col = d.tile * 16 * d.cb + c;
+    const float inv = m == -inf ? 0.0f : 1.0f / l;
+    *reinterpret_cast<float4 *>(a.out + ((size_t)(d.q0 + col / G) * a.nh + (size_t)d.kvh * G + col % G) * HD + 4 * e) =
+        make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+// What the launches take: the items at most, and whether any sequence can have
+// several chunks (from the page table's width: the lengths are on the GPU).
 struct KvAttnPlan {
-    int64_t units, items;                // column tiles, items at most
-    int32_t want;
+    int64_t items;
     bool split;
 };
 
 static KvAttnPlan kv_attn_plan(const KvAttnArgs &a)
 {
     KvAttnPlan p;
-    p.units = (int64_t)a.b.n_tokens * (a.nh / a.nkv) / KA_COLS + a.b.n_seqs;
-    p.want = (KA_ITEMS + a.nkv - 1) / a.nkv;
-    const int64_t tiles = (int64_t)a.b.max_pages * (a.c.T / 32);
-    p.split = tiles > KA_CHUNK;
-    // a column tile has at most one chunk more than its share of those wanted
-    p.items = p.split ? p.want + p.units : p.units;
+    // a sequence of c columns has at most c / 32 + 1 tiles
+    const int64_t tiles = (int64_t)a.b.n_tokens * (a.nh / a.nkv) / KA_COLS + a.b.n_seqs;
+    p.split = (int64_t)a.b.max_pages * (a.c.T / 32) > KA_CHUNK;
+    // and at most one chunk more per tile than its share of those wanted
+    p.items = tiles * a.nkv + (p.split ? KA_ITEMS : 0);
     return p;
 }
 
 size_t kv_attn_ws_bytes(const KvAttnArgs &a)
 {
     const KvAttnPlan p = kv_attn_plan(a);
-    return p.split ? (size_t)p.items * a.nkv * KA_COLS * (a.hd + 2) * 4 : 256;
+    return p.split ? (size_t)p.items * (sizeof(KvDesc) + (size_t)KA_COLS * (a.hd + 2) * 4) : 256;
 }
 
 hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
@@ -503,9 +636,9 @@ hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
     KvAttnArgs a = args;
     if (a.nkv <= 0 || a.nh % a.nkv) return hipErrorInvalidValue;
     const KvAttnPlan p = kv_attn_plan(a);
-    a.items = p.want;
+    a.items = (int32_t)p.items;
     a.split = p.split;
-    const dim3 grid((unsigned)(p.items * a.nkv)), block(KA_WAVES * 64);
+    const dim3 grid((unsigned)p.items), block(KA_WAVES * 64);
     switch (a.hd * (a.c.type == DMOE_KV_E4M3 ? -1 : 1)) {
     case 64: hipLaunchKernelGGL((k_kv_attn<64, false>), grid, block, 0, s, a); break;
     case 128: hipLaunchKernelGGL((k_kv_attn<128, false>), grid, block, 0, s, a); break;
@@ -515,11 +648,11 @@ hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.split) return e;
-    const dim3 join((unsigned)p.units, KA_COLS * a.nkv);
+    const dim3 join((unsigned)p.items, KA_COLS / KJ_COLS);
     if (a.hd == 64)
-        hipLaunchKernelGGL((k_kv_join<64>), join, block, 0, s, a);
+        hipLaunchKernelGGL((k_kv_join<64>), join, dim3(256), 0, s, a);
     else
-        hipLaunchKernelGGL((k_kv_join<128>), join, block, 0, s, a);
+        hipLaunchKernelGGL((k_kv_join<128>), join, dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
