@@ -18,6 +18,7 @@
 // probabilities (p' = 2^(s + ve - m'), at most 1 by the choice of m'), and the
 // sum takes p' 2^-ve: no operand is rescaled.  With exponents within 100 of
 // each other no p' that counts in the sum underflows.
+#include <algorithm>
 #include <type_traits>
 
 #include "dmoe_kv.h"
@@ -32,6 +33,7 @@ constexpr int KA_SLACK = 8;              // .. and may pass that by 2^KA_SLACK b
 constexpr int KA_COLS = 32;              // columns of an item at most
 constexpr int KA_CHUNK = 16;             // token tiles of a chunk at least
 constexpr int KA_ITEMS = 512;            // items wanted of a call
+constexpr int KA_WIDE = 32768;           // columns of all kv heads from which on k_kv_attn_wide runs
 
 // one 16-byte piece of cache as f16: F16 8 values, E4M3 16
 template <bool F8>
@@ -100,10 +102,10 @@ __device__ __forceinline__ int kv_token_tiles(const KvAttnArgs &a, const KvSeq &
     return (kv_cached(q.len, a.c.T, a.b.max_pages) + 31) / 32;
 }
 
-__device__ __forceinline__ int kv_col_tiles(const KvSeq &q, int G)
+__device__ __forceinline__ int kv_col_tiles(const KvAttnArgs &a, const KvSeq &q, int G)
 {
     const int cols = q.n * G, per = 16 * kv_blocks_of_tile(cols);
-    return (cols + per - 1) / per;
+    return cols > a.wide ? 0 : (cols + per - 1) / per;
 }
 
 // Item `item` of the call, or false past the last.  One wavefront, 64
@@ -113,23 +115,30 @@ __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, Kv
     const int lane = threadIdx.x & 63;
     int C = 0x7fffffff;
     if (a.split) {
-        float w = 0.0f;                  // exact enough: a length, not an index
+        float w = 0.0f, u = 0.0f;        // exact enough: a length, not an index
         for (int base = 0; base < a.b.n_seqs; base += 64)
             if (base + lane < a.b.n_seqs) {
                 const KvSeq q = kv_seq(a.b, base + lane);
-                w += (float)kv_col_tiles(q, G) * (float)kv_token_tiles(a, q);
+                const float tiles = (float)kv_col_tiles(a, q, G);
+                u += tiles;
+                w += tiles * (float)kv_token_tiles(a, q);
             }
 #pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) w += __shfl_xor(w, d, 64);
-        // rounded up beyond what the sum's rounding can hide
-        C = max(KA_CHUNK, (int)(w * (float)a.nkv / (float)KA_ITEMS * 1.001f) + 1);
+        for (int d = 32; d >= 1; d >>= 1) {
+            w += __shfl_xor(w, d, 64);
+            u += __shfl_xor(u, d, 64);
+        }
+        // a column tile's last chunk is half empty on average: so many items
+        // fewer are shared out, that all start in one round
+        const float items = fmaxf((float)KA_ITEMS - 0.5f * u * (float)a.nkv, 0.25f * (float)KA_ITEMS);
+        C = max(KA_CHUNK, (int)(w * (float)a.nkv / items) + 1);
     }
     for (int base = 0; base < a.b.n_seqs; base += 64) {
         KvSeq q{0, 0, 0};
         int tiles = 0, ks = 1;
         if (base + lane < a.b.n_seqs) {
             q = kv_seq(a.b, base + lane);
-            tiles = kv_col_tiles(q, G);
+            tiles = kv_col_tiles(a, q, G);
             // (a sequence without tokens still has its rows to zero)
             if (a.split) ks = max(1, (kv_token_tiles(a, q) + C - 1) / C);
         }
@@ -168,45 +177,66 @@ __device__ __forceinline__ float *kv_part(const KvAttnArgs &a, int item)
     return (float *)((KvDesc *)a.ws + a.items) + (size_t)item * KA_COLS * (HD + 2);
 }
 
-// One item's columns, 16 CB of them: the workgroup's wavefronts take its token
-// tiles in turn and join their results in LDS.  A tile's keys and values go
-// straight from global memory to the registers that hold them as operands; the
-// next tile's keys are loaded once a tile's scores stand, its values once its
-// sums do, so that loads are always in flight and no second set of registers
-// is needed.
+// ---------------------------------------------------------------------------
+// What a wavefront holds of its 16 CB columns, and the steps of a token tile.
 template <int HD, bool F8, int CB>
-__device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it, int G, float *s_o, float *s_m, float *s_l)
-{
-    constexpr int NC = HD / 32;                    // 32-dim chunks of a row
-    constexpr int NB = HD / 16;                    // 16-dim blocks of O
-    constexpr int EB = F8 ? 1 : 2, NE = F8 ? 2 : 1;
-    constexpr int NK = HD * EB / 32;               // 16-byte pieces a lane loads of a tile's keys, and of its values
-    constexpr int LO = HD + 4;                     // row of O in LDS: padded against bank conflicts
-    const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const KvSeq q = it.q;
-    const int kvh = it.kvh;
-    const int cached = kv_cached(q.len, a.c.T, a.b.max_pages);
-    const float inf = __builtin_inff(), low = -3.402823466e38f;
+struct KvWave {
+    static constexpr int NC = HD / 32;             // 32-dim chunks of a row
+    static constexpr int NB = HD / 16;             // 16-dim blocks of O
+    static constexpr int EB = F8 ? 1 : 2, NE = F8 ? 2 : 1;       // bytes of a value; operands that a 16-byte piece makes
+    static constexpr int NK = HD * EB / 32;        // 16-byte pieces a lane has of a tile's keys, and of its values
 
-    // this lane's columns: query q.q0 + col / G, head kvh G + col % G; tokens
-    // 0 .. vis - 1 are what it sees
-    int vis[CB], last = 0, least = cached;
+    // lane: column r16 of each 16-column block, and of the operands' 32 inner
+    // positions the 8 of group g
+    int lane, r16, g;
+    int vis[CB];                                   // tokens 0 .. vis - 1 are what a column sees
+    int least, last;                               // the least and the most of the live columns' vis
+    float cmul[CB];                                // log2(e) / sqrt(hd) over the query's power of two
+    // m: the columns' reference of s + ve, raised when a score passes it by
+    // KA_SLACK (-inf: nothing seen; at least -FLT_MAX else, so that a row whose
+    // every score is -inf ends as 0 / 0, not as empty); l: this lane's share of
+    // the sum; o: the sums of values, [block of dims], rows 4 g + i
+    float m[CB], l[CB];
+    kv_f4 o[CB][NB];
+
+    // column `col` of sequence q: query q.q0 + col / G, head kvh G + col % G
+    __device__ __forceinline__ void start(const KvAttnArgs &a, const KvSeq &q, int G, int col0)
+    {
+        lane = threadIdx.x & 63;
+        r16 = lane & 15;
+        g = lane >> 4;
+        const int cached = kv_cached(q.len, a.c.T, a.b.max_pages);
+        last = 0;
+        least = cached;
 #pragma unroll
-    for (int cb = 0; cb < CB; cb++) {
-        const int col = (it.tile * CB + cb) * 16 + r16;
-        const bool live = col < q.n * G;
-        vis[cb] = live ? kv_visible(q.len - q.n + col / G, cached, a.block) : 0;
-        last = max(last, vis[cb]);
-        if (live) least = min(least, vis[cb]);
+        for (int cb = 0; cb < CB; cb++) {
+            const int col = col0 + 16 * cb + r16;
+            const bool live = col < q.n * G;
+            vis[cb] = live ? kv_visible(q.len - q.n + col / G, cached, a.block) : 0;
+            last = max(last, vis[cb]);
+            if (live) least = min(least, vis[cb]);
+            m[cb] = -__builtin_inff();
+            l[cb] = 0.0f;
+#pragma unroll
+            for (int b = 0; b < NB; b++) o[cb][b] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int d = 8; d >= 1; d >>= 1) {
+            last = max(last, __shfl_xor(last, d, 64));
+            least = min(least, __shfl_xor(least, d, 64));
+        }
+        last = __builtin_amdgcn_readfirstlane(last);
+        least = __builtin_amdgcn_readfirstlane(least);
     }
-    // the queries as operands in LDS, [16-column block][chunk][hi, lo][lane]:
-    // every wavefront has the same, and registers are short.  Chunk 2 p + e of a
-    // lane holds dims 64 p + 16 g + 8 e .. + 7 (its 16 dims of a 64-dim half are
-    // one piece of an E4M3 key row)
-    kv_h8 *s_q = reinterpret_cast<kv_h8 *>(s_o);
-    if (w < CB) {
-        const int col = (it.tile * CB + w) * 16 + r16;
+
+    // The queries of 16 columns from col0 on as operands: put(c, hi, lo) takes
+    // chunk c.  Chunk 2 p + e of a lane holds dims 64 p + 16 g + 8 e .. + 7 (its
+    // 16 dims of a 64-dim half are one piece of an E4M3 key row).  Returns cmul.
+    template <class Put>
+    static __device__ __forceinline__ float queries(const KvAttnArgs &a, const KvSeq &q, int G, int kvh, int col0, Put &&put)
+    {
+        const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+        const int col = col0 + r16;
         const bool live = col < q.n * G;
         const int qi = live ? col / G : 0, hg = live ? col % G : 0;
         const float *src = a.q + ((size_t)(q.q0 + qi) * a.nh + (size_t)kvh * G + hg) * HD + 16 * g;
@@ -237,7 +267,6 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
             up = min(8 - ex, 100);
         }
         const float mul = ldexpf(1.0f, up);
-        if (g == 0) s_m[16 * w + r16] = ldexpf(a.scale * 1.44269504088896341f, -up);
 #pragma unroll
         for (int c = 0; c < NC; c++) {
             kv_h8 hi, lo;
@@ -247,262 +276,367 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
                 hi[j] = (_Float16)y;
                 lo[j] = (_Float16)(y - (float)hi[j]);
             }
-            s_q[((w * NC + c) * 2 + 0) * 64 + lane] = hi;
-            s_q[((w * NC + c) * 2 + 1) * 64 + lane] = lo;
+            put(c, hi, lo);
         }
-    }
-#pragma unroll
-    for (int d = 8; d >= 1; d >>= 1) {
-        last = max(last, __shfl_xor(last, d, 64));
-        least = min(least, __shfl_xor(least, d, 64));
-    }
-    last = __builtin_amdgcn_readfirstlane(last);
-    least = __builtin_amdgcn_readfirstlane(least);
-    // this wavefront's token tiles: tile0 + w, every KA_WAVES-th, up to tile1
-    const int tile0 = it.split * it.chunk, tile1 = min(tile0 + it.chunk, (last + 31) / 32);
-
-    // m: the columns' reference of s + ve, raised when a score passes it by
-    // KA_SLACK (-inf: nothing seen; at least -FLT_MAX else, so that a row whose
-    // every score is -inf ends as 0 / 0, not as empty); l: this lane's share of
-    // the sum
-    float m[CB], l[CB];
-    kv_f4 o[CB][NB];
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) {
-        m[cb] = -inf;
-        l[cb] = 0.0f;
-#pragma unroll
-        for (int b = 0; b < NB; b++) o[cb][b] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        return ldexpf(a.scale * 1.44269504088896341f, -up);
     }
 
-    // row r of key block kb is token 8 (r / 4) + 4 kb + r % 4, so that the
-    // scores of a lane are those of tokens 8 g + 4 kb + i
-    const uint32_t koff = (8 * (r16 >> 2) + (r16 & 3)) * HD * EB + 16 * EB * g;
-    const uint32_t voff = (r16 * 4 + g) * 16;
-    uint4 kr[NK], vr[NK];
-    auto load_k = [&](size_t byte) {
-        const uint8_t *K = (const uint8_t *)a.c.k + byte;
-#pragma unroll
-        for (int i = 0; i < NK; i++) {
-            // key block, then chunk (F16) or pair of chunks (E4M3)
-            const int kb = i / (NK / 2), ch = i % (NK / 2) * NE;
-            kr[i] = *reinterpret_cast<const uint4 *>(K + koff + 4 * kb * HD * EB + (64 * (ch / 2) + 8 * (ch % 2)) * EB);
-        }
+    // Where a lane's pieces of a tile lie, in bytes from the tile's keys or
+    // values.  Row r of key block kb is token 8 (r / 4) + 4 kb + r % 4, so that
+    // the scores of a lane are those of tokens 8 g + 4 kb + i.
+    __device__ __forceinline__ uint4 key_piece(const KvAttnArgs &a, size_t byte, int i) const
+    {
+        // key block, then chunk (F16) or pair of chunks (E4M3)
+        const int kb = i / (NK / 2), ch = i % (NK / 2) * NE;
+        const uint8_t *src = (const uint8_t *)a.c.k + byte + (uint32_t)((8 * (r16 >> 2) + (r16 & 3)) * HD + 16 * g) * EB;
+        return *reinterpret_cast<const uint4 *>(src + (4 * kb * HD + 64 * (ch / 2) + 8 * (ch % 2)) * EB);
+    }
+    __device__ __forceinline__ uint4 value_piece(const KvAttnArgs &a, size_t byte, int i) const
+    {
+        const uint8_t *src = (const uint8_t *)a.c.v + byte + (uint32_t)(r16 * 4 + g) * 16;
+        return *reinterpret_cast<const uint4 *>(src + 1024 * i);
+    }
+
+    // One tile of 32 tokens from k0 on.  FULL: every column sees all of it.
+    template <bool FULL>
+    struct Step {
+        kv_f4 sc[CB][2];
+        float c[CB], mt[CB];
+        int k0, ke, ve;
+        kv_h8 ph[CB], pl[CB];
     };
-    auto load_v = [&](size_t byte) {
-        const uint8_t *V = (const uint8_t *)a.c.v + byte;
-#pragma unroll
-        for (int i = 0; i < NK; i++) vr[i] = *reinterpret_cast<const uint4 *>(V + voff + 1024 * i);
-    };
+    template <bool FULL>
+    __device__ __forceinline__ bool seen(const Step<FULL> &s, int cb, int kb, int e) const
+    {
+        return FULL || s.k0 + 8 * g + 4 * kb + e < vis[cb];
+    }
 
-    __syncthreads();
-    float cmul[CB];
+    // the scores; true if one passes its column's reference by KA_SLACK
+    template <bool FULL, class Key, class Query>
+    __device__ __forceinline__ bool scores(Step<FULL> &s, Key &&key, Query &&query)
+    {
 #pragma unroll
-    for (int cb = 0; cb < CB; cb++) cmul[cb] = s_m[16 * cb + r16];
-
-    // up to 64 of the wavefront's tiles at a time: a lane looks up one tile's
-    // page and exponents, and the loop takes them from there
-    for (int base = tile0 + w; base < tile1; base += 64 * KA_WAVES) {
-        const int tt = base + KA_WAVES * lane;
-        int page = -1, kes = 0, ves = 0;
-        if (tt < tile1) page = kv_page(a.b, a.c, it.s, 32 * tt);
-        const size_t slot = ((size_t)max(page, 0) * a.nkv + kvh) * (a.c.T / 32) + tt % (a.c.T / 32);
-        if (F8 && page >= 0) {
-            kes = a.c.k_exp[slot];
-            ves = a.c.v_exp[slot];
-        }
-        const uint32_t blo = (uint32_t)(slot * 32 * HD * EB), bhi = (uint32_t)(slot * 32 * HD * EB >> 32);
-        auto where = [&](int i) {
-            return (size_t)(uint32_t)__builtin_amdgcn_readlane(bhi, i) << 32 | (uint32_t)__builtin_amdgcn_readlane(blo, i);
-        };
-        uint64_t todo = __ballot(page >= 0);
-        if (!todo) continue;
-        int i = __builtin_ctzll(todo);
-        load_k(where(i));
-        load_v(where(i));
-        // tiles while `more` of them; FULL: every column sees all of each.  The
-        // references are raised outside the loop over tiles (the tile's scores
-        // are then formed again): a conditional change of the sums inside it
-        // costs a copy of them all per tile.
-        auto run = [&](auto full, auto &&more) {
-          constexpr bool FULL = decltype(full)::value;
-          for (;;) {
-            bool raise = false;
-            float mt[CB];
-            while (more()) {
-            const int k0 = 32 * (base + KA_WAVES * i), ve = F8 ? __builtin_amdgcn_readlane(ves, i) : 0;
-            const int ke = F8 ? __builtin_amdgcn_readlane(kes, i) : 0;
-            int ql0 = lane;
-            asm volatile("" : "+v"(ql0));          // the queries are read again each tile, not kept in registers
-            kv_f4 sc[CB][2];
+        for (int cb = 0; cb < CB; cb++)
 #pragma unroll
-            for (int cb = 0; cb < CB; cb++)
+            for (int kb = 0; kb < 2; kb++) s.sc[cb][kb] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int kb = 0; kb < 2; kb++) sc[cb][kb] = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int ch = 0; ch < NC; ch += NE) {
+            kv_h8 kf[2][NE];
+            key(ch, kf);
 #pragma unroll
-            for (int ch = 0; ch < NC; ch += NE) {
-                kv_h8 kf[2][NE];
+            for (int e = 0; e < NE; e++)
 #pragma unroll
-                for (int kb = 0; kb < 2; kb++) kv_widen<F8>(kr[kb * (NK / 2) + ch / NE], kf[kb]);
-#pragma unroll
-                for (int e = 0; e < NE; e++)
+                for (int part = 0; part < 2; part++)           // the small half first
 #pragma unroll
                     for (int cb = 0; cb < CB; cb++) {
-                        const kv_h8 qh = s_q[((cb * NC + ch + e) * 2 + 0) * 64 + ql0];
-                        const kv_h8 ql = s_q[((cb * NC + ch + e) * 2 + 1) * 64 + ql0];
+                        const kv_h8 qf = query(cb, ch + e, 1 - part);
 #pragma unroll
-                        for (int kb = 0; kb < 2; kb++) {
-                            sc[cb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kb][e], ql, sc[cb][kb], 0, 0, 0);
-                            sc[cb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kb][e], qh, sc[cb][kb], 0, 0, 0);
-                        }
+                        for (int kb = 0; kb < 2; kb++)
+                            s.sc[cb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kb][e], qf, s.sc[cb][kb], 0, 0, 0);
                     }
-            }
-            auto seen = [&](int cb, int kb, int e) { return FULL || k0 + 8 * g + 4 * kb + e < vis[cb]; };
-            float c[CB];
-            bool above = false;
+        }
+        bool above = false;
 #pragma unroll
-            for (int cb = 0; cb < CB; cb++) {
-                c[cb] = F8 ? ldexpf(cmul[cb], ke) : cmul[cb];
-                float smax = -inf;
+        for (int cb = 0; cb < CB; cb++) {
+            s.c[cb] = F8 ? ldexpf(cmul[cb], s.ke) : cmul[cb];
+            float smax = -__builtin_inff();
 #pragma unroll
-                for (int kb = 0; kb < 2; kb++)
+            for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) smax = fmaxf(smax, seen(cb, kb, e) ? sc[cb][kb][e] : -inf);
-                mt[cb] = fmaxf(__builtin_fmaf(smax, c[cb], (float)ve), low);
-                if (!FULL) mt[cb] = vis[cb] > k0 ? mt[cb] : -inf;
-                above |= mt[cb] > m[cb] + (float)KA_SLACK;
-            }
-            if (__any(above)) {
-                raise = true;
-                break;
-            }
-            todo &= todo - 1;
-            // (past the last tile it is loaded again: a wait counts loads, so
-            // there must always be some)
-            if (todo) i = __builtin_ctzll(todo);
-            const size_t next = where(i);
-            load_k(next);
-            kv_h8 ph[CB], pl[CB];
+                for (int e = 0; e < 4; e++)
+                    smax = fmaxf(smax, seen<FULL>(s, cb, kb, e) ? s.sc[cb][kb][e] : -__builtin_inff());
+            s.mt[cb] = fmaxf(__builtin_fmaf(smax, s.c[cb], (float)s.ve), -3.402823466e38f);
+            if (!FULL) s.mt[cb] = vis[cb] > s.k0 ? s.mt[cb] : -__builtin_inff();
+            above |= s.mt[cb] > m[cb] + (float)KA_SLACK;
+        }
+        return __any(above);
+    }
+
+    // raises the references to what a tile's scores have met
+    __device__ __forceinline__ void raise(const float (&top)[CB])
+    {
 #pragma unroll
-            for (int cb = 0; cb < CB; cb++) {
-                const float k = (float)(ve + KA_SHIFT) - (!FULL && m[cb] == -inf ? 0.0f : m[cb]);
-                float sum = 0.0f;
+        for (int cb = 0; cb < CB; cb++) {
+            float mt = fmaxf(top[cb], __shfl_xor(top[cb], 16, 64));
+            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+            const float mn = fmaxf(m[cb], mt);
+            const float corr = m[cb] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[cb] - mn);
+            m[cb] = mn;
+            l[cb] *= corr;
 #pragma unroll
-                for (int kb = 0; kb < 2; kb++)
+            for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int e = 0; e < 4; e += 2) {
-                        kv_f2 p;
+                for (int e = 0; e < 4; e++) o[cb][b][e] *= corr;
+        }
+    }
+
+    // the probabilities, in place the operand of the second product
+    template <bool FULL>
+    __device__ __forceinline__ void weights(Step<FULL> &s)
+    {
 #pragma unroll
-                        for (int x = 0; x < 2; x++) {
-                            p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cb][kb][e + x], c[cb], k));
-                            p[x] = seen(cb, kb, e + x) ? p[x] : 0.0f;
-                            sum += p[x];
-                        }
-                        const kv_h2 hi = __builtin_convertvector(p, kv_h2), lo = kv_rest(p, hi);
-                        ph[cb][4 * kb + e] = hi[0];
-                        ph[cb][4 * kb + e + 1] = hi[1];
-                        pl[cb][4 * kb + e] = lo[0];
-                        pl[cb][4 * kb + e + 1] = lo[1];
+        for (int cb = 0; cb < CB; cb++) {
+            const float k = (float)(s.ve + KA_SHIFT) - (!FULL && m[cb] == -__builtin_inff() ? 0.0f : m[cb]);
+            float sum = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    kv_f2 p;
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(s.sc[cb][kb][e + x], s.c[cb], k));
+                        p[x] = seen<FULL>(s, cb, kb, e + x) ? p[x] : 0.0f;
+                        sum += p[x];
                     }
-                l[cb] = F8 ? __builtin_fmaf(sum, ldexpf(1.0f, -ve), l[cb]) : l[cb] + sum;
-            }
-            // values: O rows are dims 16 b + row (F16), 32 (b / 2) + 2 row + b % 2 (E4M3)
-            if (FULL) {
+                    const kv_h2 hi = __builtin_convertvector(p, kv_h2), lo = kv_rest(p, hi);
+                    s.ph[cb][4 * kb + e] = hi[0];
+                    s.ph[cb][4 * kb + e + 1] = hi[1];
+                    s.pl[cb][4 * kb + e] = lo[0];
+                    s.pl[cb][4 * kb + e + 1] = lo[1];
+                }
+            l[cb] = F8 ? __builtin_fmaf(sum, ldexpf(1.0f, -s.ve), l[cb]) : l[cb] + sum;
+        }
+    }
+
+    // o += V^T P^T.  O rows are dims 16 b + row (F16), 32 (b / 2) + 2 row + b % 2 (E4M3).
+    template <bool FULL, class Value>
+    __device__ __forceinline__ void add(Step<FULL> &s, Value &&value)
+    {
+        if (FULL) {
 #pragma unroll
-                for (int p = 0; p < NK; p++) {
-                    kv_h8 vf[NE];
-                    kv_widen<F8>(vr[p], vf);
+            for (int p = 0; p < NK; p++) {
+                kv_h8 vf[NE];
+                value(p, vf);
+#pragma unroll
+                for (int part = 0; part < 2; part++)
 #pragma unroll
                     for (int e = 0; e < NE; e++)
 #pragma unroll
-                        for (int cb = 0; cb < CB; cb++) {
-                            const int b = p * NE + e;
-                            o[cb][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[e], pl[cb], o[cb][b], 0, 0, 0);
-                            o[cb][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[e], ph[cb], o[cb][b], 0, 0, 0);
-                        }
-                }
-            } else {
-                // what a column does not see may hold anything (0 times a NaN
-                // is one), so the columns of each limit in turn add a product
-                // whose values end there
-                for (int done = k0;;) {
-                    int lim = 0x7fffffff;
+                        for (int cb = 0; cb < CB; cb++)
+                            o[cb][p * NE + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[e], part ? s.ph[cb] : s.pl[cb],
+                                                                                       o[cb][p * NE + e], 0, 0, 0);
+            }
+            return;
+        }
+        // what a column does not see may hold anything (0 times a NaN is one),
+        // so the columns of each limit in turn add a product whose values end
+        // there
+        for (int done = s.k0;;) {
+            int lim = 0x7fffffff;
 #pragma unroll
-                    for (int cb = 0; cb < CB; cb++)
-                        if (vis[cb] > done) lim = min(lim, vis[cb]);
+            for (int cb = 0; cb < CB; cb++)
+                if (vis[cb] > done) lim = min(lim, vis[cb]);
 #pragma unroll
-                    for (int d = 8; d >= 1; d >>= 1) lim = min(lim, __shfl_xor(lim, d, 64));
-                    lim = __builtin_amdgcn_readfirstlane(lim);
-                    if (lim == 0x7fffffff) break;
+            for (int d = 8; d >= 1; d >>= 1) lim = min(lim, __shfl_xor(lim, d, 64));
+            lim = __builtin_amdgcn_readfirstlane(lim);
+            if (lim == 0x7fffffff) break;
 #pragma unroll
-                    for (int p = 0; p < NK; p++) {
-                        kv_h8 vf[NE];
-                        kv_widen<F8>(vr[p], vf);
+            for (int p = 0; p < NK; p++) {
+                kv_h8 vf[NE];
+                value(p, vf);
 #pragma unroll
-                        for (int e = 0; e < NE; e++) {
-                            const kv_h8 y = kv_cut(vf[e], g, lim - k0);
+                for (int e = 0; e < NE; e++) {
+                    const kv_h8 y = kv_cut(vf[e], g, lim - s.k0);
 #pragma unroll
-                            for (int cb = 0; cb < CB; cb++) {
-                                const bool mine = vis[cb] > done && (vis[cb] == lim || lim >= k0 + 32);
-                                kv_f4 t = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
-                                t = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, pl[cb], t, 0, 0, 0);
-                                t = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, ph[cb], t, 0, 0, 0);
+                    for (int cb = 0; cb < CB; cb++) {
+                        const bool mine = vis[cb] > done && (vis[cb] == lim || lim >= s.k0 + 32);
+                        kv_f4 t = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, s.pl[cb], t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, s.ph[cb], t, 0, 0, 0);
 #pragma unroll
-                                for (int x = 0; x < 4; x++) o[cb][p * NE + e][x] += mine ? t[x] : 0.0f;
-                            }
-                        }
-                        __builtin_amdgcn_sched_barrier(0);     // one piece at a time: registers are short
+                        for (int x = 0; x < 4; x++) o[cb][p * NE + e][x] += mine ? t[x] : 0.0f;
                     }
-                    if (lim >= k0 + 32) break;
-                    done = lim;
                 }
+                __builtin_amdgcn_sched_barrier(0);             // one piece at a time: registers are short
             }
-            load_v(next);
-            }
-            if (!raise) break;
-#pragma unroll
-            for (int cb = 0; cb < CB; cb++) {
-                mt[cb] = fmaxf(mt[cb], __shfl_xor(mt[cb], 16, 64));
-                mt[cb] = fmaxf(mt[cb], __shfl_xor(mt[cb], 32, 64));
-                const float mn = fmaxf(m[cb], mt[cb]);
-                const float corr = m[cb] == -inf ? 0.0f : __builtin_amdgcn_exp2f(m[cb] - mn);
-                m[cb] = mn;
-                l[cb] *= corr;
-#pragma unroll
-                for (int b = 0; b < NB; b++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) o[cb][b][e] *= corr;
-            }
-          }
-        };
-        run(std::true_type{}, [&] { return todo && 32 * (base + KA_WAVES * i) + 32 <= least; });
-        run(std::false_type{}, [&] { return todo != 0; });
+            if (lim >= s.k0 + 32) break;
+            done = lim;
+        }
     }
 
-    // the wavefronts' results joined in LDS: [wavefront][column][dim]
-    __syncthreads();                               // the queries' place, no longer needed
-#pragma unroll
-    for (int cb = 0; cb < CB; cb++) {
-        l[cb] += __shfl_xor(l[cb], 16, 64);
-        l[cb] += __shfl_xor(l[cb], 32, 64);
-        float *dst = s_o + ((w * CB + cb) * 16 + r16) * LO;
+    // l over the lanes of a column; column r16's sums times f to dst [HD]
+    __device__ __forceinline__ float total(int cb) const
+    {
+        const float x = l[cb] + __shfl_xor(l[cb], 16, 64);
+        return x + __shfl_xor(x, 32, 64);
+    }
+    __device__ __forceinline__ void store(int cb, float f, float *dst) const
+    {
 #pragma unroll
         for (int b = 0; b < NB; b += NE)
             if constexpr (F8) {
 #pragma unroll
                 for (int i = 0; i < 4; i += 2)
                     *reinterpret_cast<float4 *>(dst + 16 * b + 8 * g + 2 * i) =
-                        make_float4(o[cb][b][i], o[cb][b + 1][i], o[cb][b][i + 1], o[cb][b + 1][i + 1]);
+                        make_float4(o[cb][b][i] * f, o[cb][b + 1][i] * f, o[cb][b][i + 1] * f, o[cb][b + 1][i + 1] * f);
             } else {
-                *reinterpret_cast<float4 *>(dst + 16 * b + 4 * g) = make_float4(o[cb][b][0], o[cb][b][1], o[cb][b][2], o[cb][b][3]);
+                *reinterpret_cast<float4 *>(dst + 16 * b + 4 * g) =
+                    make_float4(o[cb][b][0] * f, o[cb][b][1] * f, o[cb][b][2] * f, o[cb][b][3] * f);
             }
-        if (g == 0) {
-            s_m[(w * CB + cb) * 16 + r16] = m[cb];
-            s_l[(w * CB + cb) * 16 + r16] = l[cb];
+    }
+};
+
+// The token tiles of a chunk that a wavefront walks: up to 64 at a time, a lane
+// looks up the page and the exponents of one, and the loop takes them from
+// there.
+template <int HD, bool F8>
+struct KvWalk {
+    int base, step, end;                           // lane n's tile is base + step n, below end
+    int kes, ves;
+    uint32_t blo, bhi;
+    uint64_t todo;                                 // tiles still to do, by lane; `now` is the first of them (or the last)
+    int now;
+
+    __device__ __forceinline__ void look(const KvAttnArgs &a, int s, int kvh)
+    {
+        const int tt = base + step * (int)(threadIdx.x & 63);
+        int page = -1;
+        if (tt < end) page = kv_page(a.b, a.c, s, 32 * tt);
+        const size_t slot = ((size_t)max(page, 0) * a.nkv + kvh) * (a.c.T / 32) + tt % (a.c.T / 32);
+        const size_t byte = slot * 32 * HD * (F8 ? 1 : 2);
+        blo = (uint32_t)byte;
+        bhi = (uint32_t)(byte >> 32);
+        todo = __ballot(page >= 0);
+        now = todo ? __builtin_ctzll(todo) : 0;
+        kes = ves = 0;
+        if (F8 && page >= 0) {
+            kes = a.c.k_exp[slot];
+            ves = a.c.v_exp[slot];
+        }
+    }
+    // (past the last tile `now` stays: it is loaded again, since a wait counts
+    // loads and there must always be some)
+    __device__ __forceinline__ void next()
+    {
+        todo &= todo - 1;
+        if (todo) now = __builtin_ctzll(todo);
+    }
+    __device__ __forceinline__ size_t byte() const
+    {
+        return (size_t)(uint32_t)__builtin_amdgcn_readlane(bhi, now) << 32 | (uint32_t)__builtin_amdgcn_readlane(blo, now);
+    }
+    __device__ __forceinline__ int k0() const { return 32 * (base + step * now); }
+    __device__ __forceinline__ int ke() const { return F8 ? __builtin_amdgcn_readlane(kes, now) : 0; }
+    __device__ __forceinline__ int ve() const { return F8 ? __builtin_amdgcn_readlane(ves, now) : 0; }
+};
+
+// One item's columns, 16 CB of them: the workgroup's wavefronts take its token
+// tiles in turn and join their results in LDS.  A tile's keys and values go
+// straight from global memory to the registers that hold them as operands; the
+// next tile's keys are loaded once a tile's scores stand, its values once its
+// sums do, so that loads are always in flight and no second set of registers
+// is needed.
+template <int HD, bool F8, int CB>
+__device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it, int G, float *s_o, float *s_m, float *s_l)
+{
+    typedef KvWave<HD, F8, CB> Wave;
+    constexpr int NC = Wave::NC, NK = Wave::NK, NE = Wave::NE;
+    constexpr int LO = HD + 4;                     // row of O in LDS: padded against bank conflicts
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const KvSeq q = it.q;
+    const int kvh = it.kvh;
+    const float inf = __builtin_inff();
+    Wave wave;
+    wave.start(a, q, G, it.tile * CB * 16);
+
+    uint4 kr[NK], vr[NK];
+    auto load_k = [&](size_t byte) {
+#pragma unroll
+        for (int i = 0; i < NK; i++) kr[i] = wave.key_piece(a, byte, i);
+    };
+    auto load_v = [&](size_t byte) {
+#pragma unroll
+        for (int i = 0; i < NK; i++) vr[i] = wave.value_piece(a, byte, i);
+    };
+    KvWalk<HD, F8> walk;
+    walk.base = it.split * it.chunk + w;
+    walk.step = KA_WAVES;
+    walk.end = min((it.split + 1) * it.chunk, (wave.last + 31) / 32);
+    walk.look(a, it.s, kvh);
+    if (walk.todo) {
+        load_k(walk.byte());
+        load_v(walk.byte());
+    }
+    // the queries in LDS, [16-column block][chunk][hi, lo][lane]: every
+    // wavefront has the same, and registers are short
+    kv_h8 *s_q = reinterpret_cast<kv_h8 *>(s_o);
+    if (w < CB) {
+        const float c = Wave::queries(a, q, G, kvh, (it.tile * CB + w) * 16, [&](int ch, const kv_h8 &hi, const kv_h8 &lo) {
+            s_q[((w * NC + ch) * 2 + 0) * 64 + lane] = hi;
+            s_q[((w * NC + ch) * 2 + 1) * 64 + lane] = lo;
+        });
+        if (wave.g == 0) s_m[16 * w + wave.r16] = c;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int cb = 0; cb < CB; cb++) wave.cmul[cb] = s_m[16 * cb + wave.r16];
+
+    // Tiles while `more` of them.  The references are raised outside the loop
+    // over tiles (the tile's scores are then formed again): a conditional change
+    // of the sums inside it costs a copy of them all per tile.
+    auto run = [&](auto full, auto &&more) {
+        constexpr bool FULL = decltype(full)::value;
+        for (;;) {
+            float mt[CB];
+            bool raise = false;
+            while (more()) {
+                typename Wave::template Step<FULL> st;
+                st.k0 = walk.k0();
+                st.ke = walk.ke();
+                st.ve = walk.ve();
+                int at = lane;
+                asm volatile("" : "+v"(at));       // the queries are read again each tile, not kept in registers
+                if (wave.template scores<FULL>(
+                    st,
+                    [&](int ch, kv_h8(&kf)[2][NE]) {
+#pragma unroll
+                        for (int kb = 0; kb < 2; kb++) kv_widen<F8>(kr[kb * (NK / 2) + ch / NE], kf[kb]);
+                    },
+                    [&](int cb, int ch, int low) { return s_q[((cb * NC + ch) * 2 + low) * 64 + at]; })) {
+                    raise = true;
+#pragma unroll
+                    for (int cb = 0; cb < CB; cb++) mt[cb] = st.mt[cb];
+                    break;
+                }
+                walk.next();
+                const size_t next = walk.byte();
+                load_k(next);
+                wave.template weights<FULL>(st);
+                wave.template add<FULL>(st, [&](int p, kv_h8(&vf)[NE]) { kv_widen<F8>(vr[p], vf); });
+                load_v(next);
+            }
+            if (!raise) break;
+            wave.raise(mt);
+        }
+    };
+    for (;;) {
+        run(std::true_type{}, [&] { return walk.todo && walk.k0() + 32 <= wave.least; });
+        run(std::false_type{}, [&] { return walk.todo != 0; });
+        walk.base += 64 * KA_WAVES;
+        if (walk.base >= walk.end) break;
+        walk.look(a, it.s, kvh);
+        if (walk.todo) {
+            load_k(walk.byte());
+            load_v(walk.byte());
+        }
+    }
+
+    // the wavefronts' results joined in LDS: [wavefront][column][dim]
+    __syncthreads();                               // the queries' place, no longer needed
+    constexpr int COLS = 16 * CB;
+#pragma unroll
+    for (int cb = 0; cb < CB; cb++) {
+        const int c = w * COLS + 16 * cb + wave.r16;
+        const float total = wave.total(cb);
+        wave.store(cb, 1.0f, s_o + c * LO);
+        if (wave.g == 0) {
+            s_m[c] = wave.m[cb];
+            s_l[c] = total;
         }
     }
     __syncthreads();
-    constexpr int COLS = 16 * CB;
     const int cols = min(COLS, q.n * G - it.tile * COLS);
     for (int e = threadIdx.x; e < cols * (HD / 4); e += KA_WAVES * 64) {
         const int c = e / (HD / 4), d = e % (HD / 4) * 4;
@@ -531,6 +665,139 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
             *reinterpret_cast<float4 *>(part + c * HD + d) = O;
             if (d == 0) *reinterpret_cast<float2 *>(part + KA_COLS * HD + 2 * c) = make_float2(M, L);
         }
+    }
+}
+
+// Many columns of one sequence (prompts): a workgroup takes 32 KA_WAVES of
+// them, each wavefront 32, over all the tokens they see.  A token tile is
+// loaded once for all four wavefronts, a quarter by each, widened to f16 and
+// left in LDS as operands (lane-contiguous: no bank conflicts); the next tile's
+// loads are in flight during its products.  The queries stay in registers.
+template <int HD, bool F8>
+__global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
+{
+    constexpr int CB = 2;
+    typedef KvWave<HD, F8, CB> Wave;
+    constexpr int NC = Wave::NC, NK = Wave::NK, NE = Wave::NE, NB = Wave::NB;
+    constexpr int NP = NK / 2;                     // pieces of a tile that a wavefront loads (of 2 NK)
+    __shared__ __align__(16) kv_h8 s_kv[2][(2 * NC + NB) * 64];
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int G = a.nh / a.nkv, kvh = blockIdx.x % a.nkv;
+    int s, tile;
+    KvSeq q;
+    const int per = 16 * CB * KA_WAVES;
+    const int wide = a.wide;
+    // the last column tiles see the most: they start first
+    if (!kv_find(a.b, gridDim.x / a.nkv - 1 - blockIdx.x / a.nkv,
+                 [=](const KvSeq &r) { return r.n * G > wide ? (r.n * G + per - 1) / per : 0; }, s, q, tile))
+        return;
+    const int col0 = tile * per + w * 16 * CB;
+    Wave wave;
+    wave.start(a, q, G, col0);
+    const int cached = kv_cached(q.len, a.c.T, a.b.max_pages);
+    const int most = kv_visible(q.len - q.n + (min((tile + 1) * per, q.n * G) - 1) / G, cached, a.block);
+
+    uint4 r[NP];
+    auto load = [&](size_t byte) {
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+            const int i = w * NP + j;              // wavefronts 0 and 1: keys, 2 and 3: values
+            r[j] = i < NK ? wave.key_piece(a, byte, i) : wave.value_piece(a, byte, i - NK);
+        }
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int j = 0; j < NP; j++) {
+            kv_h8 x[NE];
+            kv_widen<F8>(r[j], x);
+#pragma unroll
+            for (int e = 0; e < NE; e++) s_kv[buf][((w * NP + j) * NE + e) * 64 + lane] = x[e];
+        }
+    };
+    KvWalk<HD, F8> walk;
+    walk.base = 0;
+    walk.step = 1;
+    walk.end = (most + 31) / 32;
+    walk.look(a, s, kvh);
+    if (walk.todo) load(walk.byte());
+    kv_h8 qf[CB][NC][2];
+#pragma unroll
+    for (int cb = 0; cb < CB; cb++)
+        wave.cmul[cb] = Wave::queries(a, q, G, kvh, col0 + 16 * cb, [&](int ch, const kv_h8 &hi, const kv_h8 &lo) {
+            qf[cb][ch][0] = hi;
+            qf[cb][ch][1] = lo;
+        });
+    int buf = 0;
+    stage(0);
+    __syncthreads();
+    // Every wavefront meets the same tiles and barriers: those whose columns no
+    // longer see a tile only help to load the next.
+    auto run = [&](auto full, auto &&more) {
+        constexpr bool FULL = decltype(full)::value;
+        for (;;) {
+            float mt[CB];
+            bool raise = false;
+            while (more()) {
+                typename Wave::template Step<FULL> st;
+                st.k0 = walk.k0();
+                st.ke = walk.ke();
+                st.ve = walk.ve();
+                const kv_h8 *kv = s_kv[buf];
+                if (wave.template scores<FULL>(
+                    st,
+                    [&](int ch, kv_h8(&kf)[2][NE]) {
+#pragma unroll
+                        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                            for (int e = 0; e < NE; e++) kf[kb][e] = kv[(kb * NC + ch + e) * 64 + lane];
+                    },
+                    [&](int cb, int ch, int low) { return qf[cb][ch][low]; })) {
+                    raise = true;
+#pragma unroll
+                    for (int cb = 0; cb < CB; cb++) mt[cb] = st.mt[cb];
+                    break;
+                }
+                walk.next();
+                load(walk.byte());
+                wave.template weights<FULL>(st);
+                wave.template add<FULL>(st, [&](int p, kv_h8(&vf)[NE]) {
+#pragma unroll
+                    for (int e = 0; e < NE; e++) vf[e] = kv[(2 * NC + p * NE + e) * 64 + lane];
+                });
+                buf ^= 1;
+                stage(buf);
+                __syncthreads();
+            }
+            if (!raise) break;
+            wave.raise(mt);
+        }
+    };
+    for (;;) {
+        run(std::true_type{}, [&] { return walk.todo && walk.k0() + 32 <= wave.least; });
+        run(std::false_type{}, [&] { return walk.todo && walk.k0() < wave.last; });
+        while (walk.todo) {
+            walk.next();
+            load(walk.byte());
+            buf ^= 1;
+            stage(buf);
+            __syncthreads();
+        }
+        walk.base += 64;
+        if (walk.base >= walk.end) break;
+        walk.look(a, s, kvh);
+        if (walk.todo) load(walk.byte());
+        __syncthreads();                           // the tile before is done with
+        stage(buf);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int cb = 0; cb < CB; cb++) {
+        const int col = col0 + 16 * cb + wave.r16;
+        const float L = wave.total(cb);
+        if (col >= q.n * G) continue;
+        const float inv = wave.m[cb] == -__builtin_inff() ? 0.0f : 1.0f / L;       // nothing seen: zeros
+        wave.store(cb, inv, a.out + ((size_t)(q.q0 + col / G) * a.nh + (size_t)kvh * G + col % G) * HD);
     }
 }
 
@@ -610,7 +877,8 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a)
 // What the launches take: the items at most, and whether any sequence can have
 // several chunks (from the page table's width: the lengths are on the GPU).
 struct KvAttnPlan {
-    int64_t items;
+    int64_t items, wide_items;
+    int32_t wide;                        // columns from which on a sequence is k_kv_attn_wide's
     bool split;
 };
 
@@ -618,7 +886,11 @@ static KvAttnPlan kv_attn_plan(const KvAttnArgs &a)
 {
     KvAttnPlan p;
     // a sequence of c columns has at most c / 32 + 1 tiles
-    const int64_t tiles = (int64_t)a.b.n_tokens * (a.nh / a.nkv) / KA_COLS + a.b.n_seqs;
+    const int64_t cols = (int64_t)a.b.n_tokens * (a.nh / a.nkv);
+    const bool many = cols * a.nkv >= KA_WIDE;
+    p.wide = many ? 32 * KA_WAVES : 0x7fffffff;
+    p.wide_items = many ? (cols / (32 * KA_WAVES) + a.b.n_seqs) * a.nkv : 0;
+    const int64_t tiles = many ? std::min(cols / KA_COLS, (int64_t)a.b.n_seqs * KA_WAVES) + a.b.n_seqs : cols / KA_COLS + a.b.n_seqs;
     p.split = (int64_t)a.b.max_pages * (a.c.T / 32) > KA_CHUNK;
     // and at most one chunk more per tile than its share of those wanted
     p.items = tiles * a.nkv + (p.split ? KA_ITEMS : 0);
@@ -638,7 +910,20 @@ hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
     const KvAttnPlan p = kv_attn_plan(a);
     a.items = (int32_t)p.items;
     a.split = p.split;
+    a.wide = p.wide;
     const dim3 grid((unsigned)p.items), block(KA_WAVES * 64);
+    if (p.wide_items) {
+        const dim3 g((unsigned)p.wide_items);
+        switch (a.hd * (a.c.type == DMOE_KV_E4M3 ? -1 : 1)) {
+        case 64: hipLaunchKernelGGL((k_kv_attn_wide<64, false>), g, block, 0, s, a); break;
+        case 128: hipLaunchKernelGGL((k_kv_attn_wide<128, false>), g, block, 0, s, a); break;
+        case -64: hipLaunchKernelGGL((k_kv_attn_wide<64, true>), g, block, 0, s, a); break;
+        case -128: hipLaunchKernelGGL((k_kv_attn_wide<128, true>), g, block, 0, s, a); break;
+        default: return hipErrorInvalidValue;
+        }
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
     switch (a.hd * (a.c.type == DMOE_KV_E4M3 ? -1 : 1)) {
     case 64: hipLaunchKernelGGL((k_kv_attn<64, false>), grid, block, 0, s, a); break;
     case 128: hipLaunchKernelGGL((k_kv_attn<128, false>), grid, block, 0, s, a); break;
