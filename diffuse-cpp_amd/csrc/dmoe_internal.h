@@ -267,7 +267,7 @@ struct KvAttnArgs {
     const float *q;                      // [n_tokens][nh][hd]
     float *out;
     void *ws;
-    int32_t items, split, wide;          // set by the launch
+    int32_t units, split, wide;          // set by the launch
 };
 hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t s);
 // bytes of a.ws that the launch needs; the tables are not read

@@ -18,6 +18,7 @@ namespace dmoe {
 
 typedef _Float16 kv_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 kv_h2 __attribute__((ext_vector_type(2)));
+typedef uint32_t kv_u4 __attribute__((ext_vector_type(4)));
 typedef float kv_f2 __attribute__((ext_vector_type(2)));
 typedef float kv_f4 __attribute__((ext_vector_type(4)));
 
@@ -26,15 +27,17 @@ __device__ __forceinline__ KvSeq kv_seq(const KvBatch &b, int s)
     return kv_seq_of(b.q_start[s], b.q_start[s + 1], b.kv_len[s], b.n_tokens);
 }
 
-// Inclusive prefix sum over the 64 lanes.
+// Inclusive prefix sum over the 64 lanes, by DPP.
 __device__ __forceinline__ int kv_wave_scan(int v)
 {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int u = __shfl_up(v, d, 64);
-        if (lane >= d) v += u;
-    }
+#define KV_DPP(ctrl, rows) __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, false)
+    v += KV_DPP(0x111, 0xf);             // row_shr 1, 2, 4, 8
+    v += KV_DPP(0x112, 0xf);
+    v += KV_DPP(0x114, 0xf);
+    v += KV_DPP(0x118, 0xf);
+    v += KV_DPP(0x142, 0xa);             // lane 15 of rows 0 and 2 to rows 1 and 3
+    v += KV_DPP(0x143, 0xc);             // lane 31 to rows 2 and 3
+#undef KV_DPP
     return v;
 }
 

@@ -31,7 +31,8 @@ constexpr int KA_WAVES = 4;              // wavefronts of a workgroup
 constexpr int KA_SHIFT = 4;              // probabilities are held times 2^KA_SHIFT
 constexpr int KA_SLACK = 8;              // .. and may pass that by 2^KA_SLACK before their reference is raised
 constexpr int KA_COLS = 32;              // columns of an item at most
-constexpr int KA_CHUNK = 16;             // token tiles of a chunk at least
+constexpr int KA_WHOLE = 32;             // token tiles up to which a sequence has one chunk
+constexpr int KA_CHUNK = 8;              // token tiles of a chunk at least, of longer ones
 constexpr int KA_ITEMS = 512;            // items wanted of a call
 constexpr int KA_WIDE = 32768;           // columns of all kv heads from which on k_kv_attn_wide runs
 
@@ -92,6 +93,7 @@ struct KvItem {
     int s, kvh, tile, split;             // sequence, kv head, column tile, chunk
     int cb;                              // 16-column blocks of a tile
     int ks, chunk;                       // chunks of the sequence, token tiles of each
+    int unit;                            // column tile and kv head, counted over the call
 };
 
 // 16-column blocks of a tile of a sequence with `cols` columns
@@ -113,7 +115,7 @@ __device__ __forceinline__ int kv_col_tiles(const KvAttnArgs &a, const KvSeq &q,
 __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, KvItem &it)
 {
     const int lane = threadIdx.x & 63;
-    int C = 0x7fffffff;
+    int C = 0x7fffffff, units = 0;
     if (a.split) {
         float w = 0.0f, u = 0.0f;        // exact enough: a length, not an index
         for (int base = 0; base < a.b.n_seqs; base += 64)
@@ -140,9 +142,10 @@ __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, Kv
             q = kv_seq(a.b, base + lane);
             tiles = kv_col_tiles(a, q, G);
             // (a sequence without tokens still has its rows to zero)
-            if (a.split) ks = max(1, (kv_token_tiles(a, q) + C - 1) / C);
+            const int length = kv_token_tiles(a, q);
+            if (length > KA_WHOLE) ks = (length + C - 1) / C;
         }
-        const int count = tiles * ks * a.nkv, end = kv_wave_scan(count);
+        const int count = tiles * ks * a.nkv, end = kv_wave_scan(count), before = kv_wave_scan(tiles) - tiles;
         const uint64_t past = __ballot(end > item);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -156,25 +159,27 @@ __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, Kv
             it.kvh = i % a.nkv;
             it.split = i / a.nkv % it.ks;
             it.tile = i / a.nkv / it.ks;
+            it.unit = (units + at(before) + it.tile) * a.nkv + it.kvh;
             return true;
         }
         item -= __builtin_amdgcn_readlane(end, 63);
+        units += __builtin_amdgcn_readlane(before + tiles, 63);
     }
+    it.unit = units * a.nkv;             // how many there are
     return false;
 }
 
-// The workspace of a call whose sequences can have several chunks: per item
-// what the join has to know, then its columns' sums [KA_COLS][HD] and
-// their (m, l).
+// The workspace of a call whose sequences can have several chunks: for each
+// unit what the join has to know, then per item its columns' sums
+// [KA_COLS][HD] and their (m, l).
 struct KvDesc {
-    int32_t ks, tile, kvh, q0, cols, cb;         // ks 0: no chunk, or not the first of several
-    int32_t pad[2];
+    int32_t ks, item, tile, kvh, q0, cols, cb, pad;      // item: the unit's first
 };
 
 template <int HD>
 __device__ __forceinline__ float *kv_part(const KvAttnArgs &a, int item)
 {
-    return (float *)((KvDesc *)a.ws + a.items) + (size_t)item * KA_COLS * (HD + 2);
+    return (float *)((KvDesc *)a.ws + a.units) + (size_t)item * KA_COLS * (HD + 2);
 }
 
 // ---------------------------------------------------------------------------
@@ -281,22 +286,43 @@ struct KvWave {
         return ldexpf(a.scale * 1.44269504088896341f, -up);
     }
 
+    // A tile's first byte, kept in scalar registers beside the lane's 32-bit
+    // offset (the empty asm statements): their sums, formed ahead of the loop,
+    // would take vector registers, which are short.
+    typedef const __attribute__((address_space(1))) uint8_t *Bytes;
+    typedef const __attribute__((address_space(1))) kv_u4 *Piece;
+    static __device__ __forceinline__ Bytes at(const void *p, size_t byte)
+    {
+        Bytes tile = (Bytes)(uintptr_t)p + byte;
+        asm volatile("" : "+s"(tile));
+        return tile;
+    }
+
     // Where a lane's pieces of a tile lie, in bytes from the tile's keys or
     // values.  Row r of key block kb is token 8 (r / 4) + 4 kb + r % 4, so that
     // the scores of a lane are those of tokens 8 g + 4 kb + i.
-    __device__ __forceinline__ uint4 key_piece(const KvAttnArgs &a, size_t byte, int i) const
+    __device__ __forceinline__ uint32_t key_at() const
+    {
+        uint32_t at = ((8 * (r16 >> 2) + (r16 & 3)) * HD + 16 * g) * EB;
+        asm volatile("" : "+v"(at));
+        return at;
+    }
+    __device__ __forceinline__ uint32_t value_at() const
+    {
+        uint32_t at = (r16 * 4 + g) * 16;
+        asm volatile("" : "+v"(at));
+        return at;
+    }
+    static __device__ __forceinline__ uint4 key_piece(Bytes tile, uint32_t at, int i)
     {
         // key block, then chunk (F16) or pair of chunks (E4M3)
         const int kb = i / (NK / 2), ch = i % (NK / 2) * NE;
-        const uint8_t *src = (const uint8_t *)a.c.k + byte + (uint32_t)((8 * (r16 >> 2) + (r16 & 3)) * HD + 16 * g) * EB;
-        return *reinterpret_cast<const uint4 *>(src + (4 * kb * HD + 64 * (ch / 2) + 8 * (ch % 2)) * EB);
+        return __builtin_bit_cast(uint4, *(Piece)(tile + at + (4 * kb * HD + 64 * (ch / 2) + 8 * (ch % 2)) * EB));
     }
-    __device__ __forceinline__ uint4 value_piece(const KvAttnArgs &a, size_t byte, int i) const
+    static __device__ __forceinline__ uint4 value_piece(Bytes tile, uint32_t at, int i)
     {
-        const uint8_t *src = (const uint8_t *)a.c.v + byte + (uint32_t)(r16 * 4 + g) * 16;
-        return *reinterpret_cast<const uint4 *>(src + 1024 * i);
+        return __builtin_bit_cast(uint4, *(Piece)(tile + at + 1024 * i));
     }
-
     // One tile of 32 tokens from k0 on.  FULL: every column sees all of it.
     template <bool FULL>
     struct Step {
@@ -334,6 +360,7 @@ struct KvWave {
                         for (int kb = 0; kb < 2; kb++)
                             s.sc[cb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[kb][e], qf, s.sc[cb][kb], 0, 0, 0);
                     }
+            if (!F8 && ch == NC / 2 - 1) __builtin_amdgcn_sched_barrier(0);    // else every query operand is read ahead
         }
         bool above = false;
 #pragma unroll
@@ -352,14 +379,19 @@ struct KvWave {
         return __any(above);
     }
 
+    // the maximum over the lanes of a column
+    __device__ __forceinline__ float column_max(float x) const
+    {
+        x = fmaxf(x, __shfl_xor(x, 16, 64));
+        return fmaxf(x, __shfl_xor(x, 32, 64));
+    }
+
     // raises the references to what a tile's scores have met
     __device__ __forceinline__ void raise(const float (&top)[CB])
     {
 #pragma unroll
         for (int cb = 0; cb < CB; cb++) {
-            float mt = fmaxf(top[cb], __shfl_xor(top[cb], 16, 64));
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-            const float mn = fmaxf(m[cb], mt);
+            const float mn = fmaxf(m[cb], column_max(top[cb]));
             const float corr = m[cb] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[cb] - mn);
             m[cb] = mn;
             l[cb] *= corr;
@@ -403,11 +435,12 @@ struct KvWave {
     template <bool FULL, class Value>
     __device__ __forceinline__ void add(Step<FULL> &s, Value &&value)
     {
+        constexpr std::integral_constant<bool, FULL> full{};
         if (FULL) {
 #pragma unroll
             for (int p = 0; p < NK; p++) {
                 kv_h8 vf[NE];
-                value(p, vf);
+                value(full, p, vf);
 #pragma unroll
                 for (int part = 0; part < 2; part++)
 #pragma unroll
@@ -419,9 +452,23 @@ struct KvWave {
             }
             return;
         }
-        // what a column does not see may hold anything (0 times a NaN is one),
-        // so the columns of each limit in turn add a product whose values end
-        // there
+        // What a column does not see may hold anything, and 0 times a NaN is
+        // one: tokens that no column sees are set to zero, and if the others are
+        // not all finite, the columns of each limit in turn add a product whose
+        // values end there.
+        // (Any that is not makes a product with zeros NaN.)
+        const kv_h8 zero = {};
+        kv_f4 probe = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int p = 0; p < NK; p++) {
+            kv_h8 vf[NE];
+            value(full, p, vf);
+#pragma unroll
+            for (int e = 0; e < NE; e++)
+                probe = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv_cut(vf[e], g, last - s.k0), zero, probe, 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);                 // one piece at a time: registers are short
+        }
+        const bool one = __all(probe[0] + probe[1] + probe[2] + probe[3] == 0.0f);
         for (int done = s.k0;;) {
             int lim = 0x7fffffff;
 #pragma unroll
@@ -429,18 +476,18 @@ struct KvWave {
                 if (vis[cb] > done) lim = min(lim, vis[cb]);
 #pragma unroll
             for (int d = 8; d >= 1; d >>= 1) lim = min(lim, __shfl_xor(lim, d, 64));
-            lim = __builtin_amdgcn_readfirstlane(lim);
+            lim = one ? last : __builtin_amdgcn_readfirstlane(lim);
             if (lim == 0x7fffffff) break;
 #pragma unroll
             for (int p = 0; p < NK; p++) {
                 kv_h8 vf[NE];
-                value(p, vf);
+                value(full, p, vf);
 #pragma unroll
                 for (int e = 0; e < NE; e++) {
                     const kv_h8 y = kv_cut(vf[e], g, lim - s.k0);
 #pragma unroll
                     for (int cb = 0; cb < CB; cb++) {
-                        const bool mine = vis[cb] > done && (vis[cb] == lim || lim >= s.k0 + 32);
+                        const bool mine = one || (vis[cb] > done && (vis[cb] == lim || lim >= s.k0 + 32));
                         kv_f4 t = kv_f4{0.0f, 0.0f, 0.0f, 0.0f};
                         t = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, s.pl[cb], t, 0, 0, 0);
                         t = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, s.ph[cb], t, 0, 0, 0);
@@ -448,9 +495,9 @@ struct KvWave {
                         for (int x = 0; x < 4; x++) o[cb][p * NE + e][x] += mine ? t[x] : 0.0f;
                     }
                 }
-                __builtin_amdgcn_sched_barrier(0);             // one piece at a time: registers are short
+                __builtin_amdgcn_sched_barrier(0);
             }
-            if (lim >= s.k0 + 32) break;
+            if (one || lim >= s.k0 + 32) break;
             done = lim;
         }
     }
@@ -543,12 +590,16 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
 
     uint4 kr[NK], vr[NK];
     auto load_k = [&](size_t byte) {
+        const typename Wave::Bytes tile = Wave::at(a.c.k, byte);
+        const uint32_t at = wave.key_at();
 #pragma unroll
-        for (int i = 0; i < NK; i++) kr[i] = wave.key_piece(a, byte, i);
+        for (int i = 0; i < NK; i++) kr[i] = Wave::key_piece(tile, at, i);
     };
     auto load_v = [&](size_t byte) {
+        const typename Wave::Bytes tile = Wave::at(a.c.v, byte);
+        const uint32_t at = wave.value_at();
 #pragma unroll
-        for (int i = 0; i < NK; i++) vr[i] = wave.value_piece(a, byte, i);
+        for (int i = 0; i < NK; i++) vr[i] = Wave::value_piece(tile, at, i);
     };
     KvWalk<HD, F8> walk;
     walk.base = it.split * it.chunk + w;
@@ -602,9 +653,15 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
                 }
                 walk.next();
                 const size_t next = walk.byte();
-                load_k(next);
+                if (FULL) load_k(next);            // (registers are short in the other path, and its tiles few)
                 wave.template weights<FULL>(st);
-                wave.template add<FULL>(st, [&](int p, kv_h8(&vf)[NE]) { kv_widen<F8>(vr[p], vf); });
+                wave.template add<FULL>(st, [&](auto once, int p, kv_h8(&vf)[NE]) {
+                    uint4 x = vr[p];
+                    // (used again per limit: not to be kept widened in between)
+                    if (!once && F8) asm volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w));
+                    kv_widen<F8>(x, vf);
+                });
+                if (!FULL) load_k(next);
                 load_v(next);
             }
             if (!raise) break;
@@ -699,12 +756,13 @@ __global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
     const int most = kv_visible(q.len - q.n + (min((tile + 1) * per, q.n * G) - 1) / G, cached, a.block);
 
     uint4 r[NP];
+    // wavefronts 0 and 1: keys, 2 and 3: values
     auto load = [&](size_t byte) {
+        const typename Wave::Bytes tile = Wave::at(w < KA_WAVES / 2 ? a.c.k : a.c.v, byte);
+        const uint32_t at = w < KA_WAVES / 2 ? wave.key_at() : wave.value_at();
 #pragma unroll
-        for (int j = 0; j < NP; j++) {
-            const int i = w * NP + j;              // wavefronts 0 and 1: keys, 2 and 3: values
-            r[j] = i < NK ? wave.key_piece(a, byte, i) : wave.value_piece(a, byte, i - NK);
-        }
+        for (int j = 0; j < NP; j++)
+            r[j] = w < KA_WAVES / 2 ? Wave::key_piece(tile, at, w * NP + j) : Wave::value_piece(tile, at, w * NP + j - NK);
     };
     auto stage = [&](int buf) {
 #pragma unroll
@@ -761,9 +819,11 @@ __global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
                 walk.next();
                 load(walk.byte());
                 wave.template weights<FULL>(st);
-                wave.template add<FULL>(st, [&](int p, kv_h8(&vf)[NE]) {
+                wave.template add<FULL>(st, [&](auto once, int p, kv_h8(&vf)[NE]) {
+                    int at = lane;
+                    if (!once) asm volatile("" : "+v"(at));
 #pragma unroll
-                    for (int e = 0; e < NE; e++) vf[e] = kv[(2 * NC + p * NE + e) * 64 + lane];
+                    for (int e = 0; e < NE; e++) vf[e] = kv[(2 * NC + p * NE + e) * 64 + at];
                 });
                 buf ^= 1;
                 stage(buf);
@@ -808,40 +868,41 @@ __global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn(KvAttnArgs a)
     __shared__ float s_m[KA_WAVES * KA_COLS], s_l[KA_WAVES * KA_COLS];
     const int G = a.nh / a.nkv;
     KvItem it;
-    const bool some = kv_item(a, G, blockIdx.x, it);
-    if (a.split && threadIdx.x == 0) {
-        KvDesc d{};
-        if (some && it.split == 0 && it.ks > 1)
-            d = KvDesc{it.ks, it.tile, it.kvh, it.q.q0, min(16 * it.cb, it.q.n * G - it.tile * 16 * it.cb), it.cb, {}};
-        ((KvDesc *)a.ws)[blockIdx.x] = d;
+    if (!kv_item(a, G, blockIdx.x, it)) {
+        // at least as many items as units stay empty (the launch's bound): each
+        // item past the last marks one of those
+        const int u = it.unit + (gridDim.x - 1 - blockIdx.x);
+        if (a.split && threadIdx.x == 0 && u < a.units) ((KvDesc *)a.ws)[u].ks = 0;
+        return;
     }
-    if (!some) return;
+    if (a.split && it.split == 0 && threadIdx.x == 0)
+        ((KvDesc *)a.ws)[it.unit] = KvDesc{it.ks, (int)blockIdx.x, it.tile, it.kvh, it.q.q0,
+                                           min(16 * it.cb, it.q.n * G - it.tile * 16 * it.cb), it.cb, 0};
     if (it.cb == 1)
         kv_attend<HD, F8, 1>(a, it, G, s_o, s_m, s_l);
     else
         kv_attend<HD, F8, 2>(a, it, G, s_o, s_m, s_l);
 }
 
-// Joins the chunks of a column tile: a workgroup takes KJ_COLS of its columns,
-// its threads four dims of a column and every KJ_PARTS-th chunk.
-constexpr int KJ_COLS = 2;
-template <int HD>
-__global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a)
+// Joins the chunks of a unit: a workgroup takes COLS of its columns, its
+// threads four dims of a column and every PARTS-th chunk.
+template <int HD, int COLS, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_kv_join(KvAttnArgs a)
 {
-    constexpr int ND = HD / 4, PARTS = 256 / (KJ_COLS * ND);
-    __shared__ __align__(16) float4 s_o[PARTS][KJ_COLS][ND];
-    __shared__ float s_m[PARTS][KJ_COLS], s_l[PARTS][KJ_COLS];
+    constexpr int ND = HD / 4, PARTS = THREADS / (COLS * ND);
+    __shared__ __align__(16) float4 s_o[PARTS][COLS][ND];
+    __shared__ float s_m[PARTS][COLS], s_l[PARTS][COLS];
     const KvDesc d = ((const KvDesc *)a.ws)[blockIdx.x];
-    const int c0 = blockIdx.y * KJ_COLS;
-    if (d.ks == 0 || c0 >= d.cols) return;
-    const int e = threadIdx.x % ND, ci = threadIdx.x / ND % KJ_COLS, part = threadIdx.x / (ND * KJ_COLS);
+    const int c0 = blockIdx.y * COLS;
+    if (d.ks <= 1 || c0 >= d.cols) return;
+    const int e = threadIdx.x % ND, ci = threadIdx.x / ND % COLS, part = threadIdx.x / (ND * COLS);
     const int c = min(c0 + ci, d.cols - 1);
     const float inf = __builtin_inff();
     float m = -inf, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
     for (int j = part; j < d.ks; j += PARTS) {
-        const float *p = kv_part<HD>(a, blockIdx.x + j * a.nkv);
+        const float *p = kv_part<HD>(a, d.item + j * a.nkv);
         const float2 ml = *reinterpret_cast<const float2 *>(p + KA_COLS * HD + 2 * c);
         const float4 x = *reinterpret_cast<const float4 *>(p + c * HD + 4 * e);
         const float mn = fmaxf(m, ml.x);
@@ -877,7 +938,7 @@ __global__ __launch_bounds__(256) void k_kv_join(KvAttnArgs a)
 // What the launches take: the items at most, and whether any sequence can have
 // several chunks (from the page table's width: the lengths are on the GPU).
 struct KvAttnPlan {
-    int64_t items, wide_items;
+    int64_t items, units, wide_items;    // items and units of k_kv_attn at most, items of k_kv_attn_wide
     int32_t wide;                        // columns from which on a sequence is k_kv_attn_wide's
     bool split;
 };
@@ -885,22 +946,25 @@ struct KvAttnPlan {
 static KvAttnPlan kv_attn_plan(const KvAttnArgs &a)
 {
     KvAttnPlan p;
-    // a sequence of c columns has at most c / 32 + 1 tiles
-    const int64_t cols = (int64_t)a.b.n_tokens * (a.nh / a.nkv);
+    const int64_t cols = (int64_t)a.b.n_tokens * (a.nh / a.nkv), seqs = a.b.n_seqs;
     const bool many = cols * a.nkv >= KA_WIDE;
-    p.wide = many ? 32 * KA_WAVES : 0x7fffffff;
-    p.wide_items = many ? (cols / (32 * KA_WAVES) + a.b.n_seqs) * a.nkv : 0;
-    const int64_t tiles = many ? std::min(cols / KA_COLS, (int64_t)a.b.n_seqs * KA_WAVES) + a.b.n_seqs : cols / KA_COLS + a.b.n_seqs;
-    p.split = (int64_t)a.b.max_pages * (a.c.T / 32) > KA_CHUNK;
-    // and at most one chunk more per tile than its share of those wanted
-    p.items = tiles * a.nkv + (p.split ? KA_ITEMS : 0);
+    p.wide = many ? (seqs == 1 ? 0 : 32 * KA_WAVES) : 0x7fffffff;
+    p.wide_items = many ? (cols / (32 * KA_WAVES) + seqs) * a.nkv : 0;
+    // a sequence of c columns has at most c / 32 + 1 column tiles
+    int64_t tiles = cols / KA_COLS + seqs;
+    if (many) tiles = std::min(tiles, seqs * (KA_WAVES + 1));
+    if (p.wide == 0) tiles = 0;
+    p.units = tiles * a.nkv;
+    p.split = tiles > 0 && (int64_t)a.b.max_pages * (a.c.T / 32) > KA_WHOLE;
+    // chunks: less than one more per unit than its share of those wanted
+    p.items = p.units + (p.split ? KA_ITEMS : 0);
     return p;
 }
 
 size_t kv_attn_ws_bytes(const KvAttnArgs &a)
 {
     const KvAttnPlan p = kv_attn_plan(a);
-    return p.split ? (size_t)p.items * (sizeof(KvDesc) + (size_t)KA_COLS * (a.hd + 2) * 4) : 256;
+    return p.split ? (size_t)p.units * sizeof(KvDesc) + (size_t)p.items * KA_COLS * (a.hd + 2) * 4 : 256;
 }
 
 hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
@@ -908,7 +972,7 @@ hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
     KvAttnArgs a = args;
     if (a.nkv <= 0 || a.nh % a.nkv) return hipErrorInvalidValue;
     const KvAttnPlan p = kv_attn_plan(a);
-    a.items = (int32_t)p.items;
+    a.units = (int32_t)p.units;
     a.split = p.split;
     a.wide = p.wide;
     const dim3 grid((unsigned)p.items), block(KA_WAVES * 64);
@@ -924,6 +988,7 @@ hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
+    if (!p.items) return hipSuccess;
     switch (a.hd * (a.c.type == DMOE_KV_E4M3 ? -1 : 1)) {
     case 64: hipLaunchKernelGGL((k_kv_attn<64, false>), grid, block, 0, s, a); break;
     case 128: hipLaunchKernelGGL((k_kv_attn<128, false>), grid, block, 0, s, a); break;
@@ -933,11 +998,20 @@ hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.split) return e;
-    const dim3 join((unsigned)p.items, KA_COLS / KJ_COLS);
-    if (a.hd == 64)
-        hipLaunchKernelGGL((k_kv_join<64>), join, dim3(256), 0, s, a);
+    // Few units have many chunks each (KA_ITEMS in all): a workgroup per column
+    // then, 16 or 32 chunks at a time; else one per four columns, two or four at a
+    // time, as most of a launch that has a workgroup for every column a unit
+    // could have only starts and ends.
+    const bool deep = p.units <= 32;
+    const dim3 join((unsigned)p.units, deep ? KA_COLS : KA_COLS / 4), threads(deep ? 512 : 256);
+    if (a.hd == 64 && deep)
+        hipLaunchKernelGGL((k_kv_join<64, 1, 512>), join, threads, 0, s, a);
+    else if (a.hd == 64)
+        hipLaunchKernelGGL((k_kv_join<64, 4, 256>), join, threads, 0, s, a);
+    else if (deep)
+        hipLaunchKernelGGL((k_kv_join<128, 1, 512>), join, threads, 0, s, a);
     else
-        hipLaunchKernelGGL((k_kv_join<128>), join, dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_kv_join<128, 4, 256>), join, threads, 0, s, a);
     return hipGetLastError();
 }
 
