@@ -18,6 +18,7 @@
 // and lets a block's exponent grow: rows that begin inside a block keep the
 // tokens before them, whose codes are divided by 2^(e - e_old) (exact, but for
 // codes that fall under 2^-6) where e exceeds theirs.
+#include "dmoe_device.h"
 #include "dmoe_kv.h"
 
 #pragma clang fp contract(off)
@@ -25,6 +26,10 @@
 namespace dmoe {
 
 constexpr int KA_WAVES = 4;
+
+struct __attribute__((packed, aligned(4))) Quad {
+    float x[4];
+};
 
 // f32 -> E4M3 (round to nearest even); what the type does not hold (inf, NaN,
 // and values over 448, which only KV_EMAX lets through) becomes its NaN.
@@ -34,6 +39,50 @@ __device__ __forceinline__ uint32_t kv_e4m3x2(float a, float b)
     a = fabsf(a) <= 448.0f ? a : nan;
     b = fabsf(b) <= 448.0f ? b : nan;
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
+}
+
+// cos and sin of an angle in turns: reduced exactly to an eighth of a turn and a
+// quadrant, then their Taylor series to the 16th and 17th power (the next terms
+// are below 2^-58).
+__device__ __forceinline__ double2 kv_cos_sin(double turns)
+{
+    turns -= rint(turns);
+    const double k = rint(4.0 * turns);
+    const double x = (turns - 0.25 * k) * 6.283185307179586477, z = x * x;
+    double s = 1.0 / 355687428096000.0, c = 1.0 / 20922789888000.0;
+    s = __builtin_fma(-s, z, 1.0 / 1307674368000.0);
+    c = __builtin_fma(-c, z, 1.0 / 87178291200.0);
+    s = __builtin_fma(-s, z, 1.0 / 6227020800.0);
+    c = __builtin_fma(-c, z, 1.0 / 479001600.0);
+    s = __builtin_fma(-s, z, 1.0 / 39916800.0);
+    c = __builtin_fma(-c, z, 1.0 / 3628800.0);
+    s = __builtin_fma(-s, z, 1.0 / 362880.0);
+    c = __builtin_fma(-c, z, 1.0 / 40320.0);
+    s = __builtin_fma(-s, z, 1.0 / 5040.0);
+    c = __builtin_fma(-c, z, 1.0 / 720.0);
+    s = __builtin_fma(-s, z, 1.0 / 120.0);
+    c = __builtin_fma(-c, z, 1.0 / 24.0);
+    s = __builtin_fma(-s, z, 1.0 / 6.0);
+    c = __builtin_fma(-c, z, 0.5);
+    s = __builtin_fma(-s, z, 1.0) * x;
+    c = __builtin_fma(-c, z, 1.0);
+    const int q = (int)k & 3;
+    const double cc = q & 1 ? s : c, ss = q & 1 ? c : s;
+    return make_double2(q == 1 || q == 2 ? -cc : cc, q >= 2 ? -ss : ss);
+}
+
+// The sum over a row's 16 lanes, in every one of them.
+__device__ __forceinline__ double kv_row_sum(double v)
+{
+#define KV_ROR(n) \
+    v += __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), 0x120 + n, 0xf, 0xf, false), \
+                          __builtin_amdgcn_update_dpp(0, __double2loint(v), 0x120 + n, 0xf, 0xf, false))
+    KV_ROR(8);
+    KV_ROR(4);
+    KV_ROR(2);
+    KV_ROR(1);
+#undef KV_ROR
+    return v;
 }
 
 // The least e with amax <= 448 * 2^e, in KV_EMIN .. KV_EMAX.  amax finite.
@@ -46,19 +95,20 @@ __device__ __forceinline__ int kv_exponent(float amax)
     return min(max(e, KV_EMIN), KV_EMAX);
 }
 
-// One workgroup: one block's rows (up to 32) of KA_WAVES heads.  A wavefront
+// One workgroup: one block's rows (up to 32) of `group` heads.  A wavefront
 // takes up to eight rows of a head, so 1, 2 or 4 of them share a head by the
-// block's rows and the heads take 1, 2 or 4 passes; the cosines and sines of
-// the rows are formed once for all of them.  A lane holds two dims of a row
-// (hd 64: a wavefront two rows at a time).
+// block's rows, and the group's heads take one or more passes; the cosines and
+// sines of the rows are formed once for all of them.  16 lanes hold a row, four
+// dims of each 64 a lane (16-byte loads; the norm's sum takes four DPP steps for
+// four rows at once).
 template <int HD, bool F8>
 __global__ __launch_bounds__(KA_WAVES * 64) void k_kv_append(KvAppendArgs a)
 {
-    constexpr int TPW = 128 / HD;                  // rows per wavefront step
-    constexpr int STEPS = 8 / TPW;
+    constexpr int NV = HD / 64;                    // vectors of four dims of a lane
     constexpr int EB = F8 ? 1 : 2;
-    constexpr int LROW = HD * EB + 16;             // bytes of a row in the tile
+    constexpr int LROW = HD * EB + 16;             // bytes of a row in the values' tile
     __shared__ __align__(16) uint8_t s_tile[32 * LROW];
+    __shared__ __align__(16) double s_x[KA_WAVES][4 * HD];           // rows of a step, for the rotation's partners
     __shared__ float s_amax[KA_WAVES];
     extern __shared__ __align__(16) double2 s_rot[];                 // [rows][rd / 2]
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -85,114 +135,164 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv_append(KvAppendArgs a)
     const int end = off + m;
     const int page = kv_page(a.b, a.c, s, pos);
 
-    // cos and sin of position * base^(-2 i / rd): the angle in turns, reduced
-    // to half a turn exactly
-    for (int i = threadIdx.x; i < m * half; i += KA_WAVES * 64) {
-        const int t = i / half, p = i % half;
-        double turns = (double)(pos + t) * (exp2(a.log2_step * (double)p) * 0.15915494309189533577);
-        turns -= rint(turns);
-        double sn, cs;
-        sincospi(2.0 * turns, &sn, &cs);
-        s_rot[i] = make_double2(cs, sn);
-    }
-    __syncthreads();
-
     const int share = m <= 8 ? 1 : m <= 16 ? 2 : 4;                  // wavefronts of a head
     const int rg = w & (share - 1), r0 = 8 * rg;
     uint8_t *tile = s_tile + (w / share) * share * 8 * LROW;         // rows of this wavefront's head
-    const int sub = lane / (HD / 2), d0 = 2 * (lane % (HD / 2));
-    // the rotation's partner of each of the lane's dims
-    auto partner = [&](int d) { return d < half ? d + half : d < 2 * half ? d - half : d; };
-    const int p0 = partner(d0), p1 = partner(d0 + 1);
+    const int sub = lane >> 4, d0 = 4 * (lane & 15);                 // row of a step; dims d0 + 64 v ..
     const size_t row_floats = (size_t)heads * HD;
+    const int head0 = blockIdx.y * a.group, head1 = min(head0 + a.group, heads);
+    const bool rotates = head0 < a.nh + a.nkv, caches = head1 > a.nh;
 
-    for (int pass = 0; pass < share; pass++) {
-        const int hh = (blockIdx.y * KA_WAVES) + pass * (KA_WAVES / share) + w / share;
-        const bool rotated = hh < a.nh + a.nkv, cached = hh >= a.nh && hh < heads && page >= 0;
-        const bool is_v = !rotated;
-        float v[STEPS][2];
-        float amax = 0.0f;
-        if (hh < heads) {
-            const float *src = a.qkv + (size_t)row * row_floats + (size_t)hh * HD + d0;
+    float x[2][NV][4], next[2][NV][4];
+    auto load = [&](float (&x)[2][NV][4], int hh) {
 #pragma unroll
-            for (int u = 0; u < STEPS; u++) {
-                const int t = r0 + u * TPW + sub;
-                float2 x = make_float2(0.0f, 0.0f);
-                if (t < m) {
-                    x = *reinterpret_cast<const float2 *>(src + (size_t)t * row_floats);
+        for (int u = 0; u < 2; u++) {
+            const int t = r0 + 4 * u + sub;
+            const float *src = a.qkv + (size_t)(row + t) * row_floats + (size_t)hh * HD + d0;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (t < m && hh < head1) {
+                    y = *reinterpret_cast<const float4 *>(src + 64 * v);
                     for (int k = 1; k < a.ks; k++) {   // the projection's reduction slices, in order
-                        const float2 y = *reinterpret_cast<const float2 *>(src + (size_t)k * a.kstride + (size_t)t * row_floats);
-                        x.x = x.x + y.x;
-                        x.y = x.y + y.y;
+                        const float4 z = *reinterpret_cast<const float4 *>(src + 64 * v + (size_t)k * a.kstride);
+                        y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
                     }
                 }
-                v[u][0] = x.x;
-                v[u][1] = x.y;
+                x[u][v][0] = y.x;
+                x[u][v][1] = y.y;
+                x[u][v][2] = y.z;
+                x[u][v][3] = y.w;
             }
-            if (rotated) {
-                float g0 = 1.0f, g1 = 1.0f;
+        }
+    };
+    load(x, head0 + w / share);
+
+    // cos and sin of position * base^(-2 i / rd).  A thread forms those of one
+    // pair's first row and, by rotating on, of every rows_apart-th row after it
+    if (rotates && half) {
+        const int p = threadIdx.x % half, rows_apart = KA_WAVES * 64 / half;
+        const double turn = exp2(a.log2_step * (double)p) * 0.15915494309189533577;
+        int t = threadIdx.x / half;
+        if (t < min(m, rows_apart)) {
+            double2 r = kv_cos_sin((double)(pos + t) * turn), d = make_double2(1.0, 0.0);
+            if (m > rows_apart) d = kv_cos_sin((double)rows_apart * turn);
+            for (; t < m; t += rows_apart) {
+                s_rot[t * half + p] = r;
+                r = make_double2(__builtin_fma(r.x, d.x, -(r.y * d.y)), __builtin_fma(r.x, d.y, r.y * d.x));
+            }
+        }
+    }
+    __syncthreads();
+
+    for (int hb = head0; hb < head1; hb += KA_WAVES / share) {
+        const int hh = hb + w / share;
+        load(next, hh + KA_WAVES / share);                           // the next pass's rows, in flight from here on
+        auto advance = [&]() {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int v = 0; v < NV; v++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) x[u][v][j] = next[u][v][j];
+        };
+        const bool mine = hh < head1, is_v = hh >= a.nh + a.nkv, cached = mine && hh >= a.nh && page >= 0;
+        if (mine && !is_v) {
+            double g[NV][4];
+            const float *gain = hh < a.nh ? a.q_norm : a.k_norm;
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                Quad c = {{1.0f, 1.0f, 1.0f, 1.0f}};
+                if (a.qk_norm) c = *reinterpret_cast<const Quad *>(gain + 64 * v + d0);
+#pragma unroll
+                for (int j = 0; j < 4; j++) g[v][j] = (double)c.x[j];
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int t = r0 + 4 * u + sub;
+                if (r0 + 4 * u >= m) break;
+                double y[NV][4];
+#pragma unroll
+                for (int v = 0; v < NV; v++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) y[v][j] = (double)x[u][v][j];
                 if (a.qk_norm) {
-                    const float *gain = hh < a.nh ? a.q_norm : a.k_norm;
-                    g0 = gain[d0];
-                    g1 = gain[d0 + 1];
+                    double ss = 0.0;
+#pragma unroll
+                    for (int v = 0; v < NV; v++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) ss = __builtin_fma(y[v][j], y[v][j], ss);
+                    ss = kv_row_sum(ss);
+                    const double scale = 1.0 / sqrt(ss / (double)HD + (double)a.eps);
+#pragma unroll
+                    for (int v = 0; v < NV; v++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) y[v][j] *= scale * g[v][j];
+                }
+                if (half) {
+                    double *sx = &s_x[w][sub * HD];
+                    __builtin_amdgcn_wave_barrier();
+                    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+#pragma unroll
+                    for (int v = 0; v < NV; v++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) sx[64 * v + d0 + j] = y[v][j];
+                    __builtin_amdgcn_wave_barrier();
+                    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+                    const double2 *rot = s_rot + min(t, m - 1) * half;
+#pragma unroll
+                    for (int v = 0; v < NV; v++) {
+                        if (64 * v >= 2 * half) break;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int d = 64 * v + d0 + j;
+                            const bool in = d < 2 * half, second = d >= half;
+                            const double2 r = rot[in ? (second ? d - half : d) : 0];
+                            const double z = sx[in ? (second ? d - half : d + half) : 0];
+                            const double to = __builtin_fma(second ? z : -z, r.y, y[v][j] * r.x);
+                            y[v][j] = in ? to : y[v][j];
+                        }
+                    }
                 }
 #pragma unroll
-                for (int u = 0; u < STEPS; u++) {
-                    const int t = r0 + u * TPW + sub;
-                    double y0 = v[u][0], y1 = v[u][1];
-                    if (a.qk_norm) {
-                        double ss = y0 * y0 + y1 * y1;
+                for (int v = 0; v < NV; v++) {
 #pragma unroll
-                        for (int d = HD / 4; d >= 1; d >>= 1) ss += __shfl_xor(ss, d, 64);
-                        const double scale = 1.0 / sqrt(ss / (double)HD + (double)a.eps);
-                        y0 = y0 * scale * (double)g0;
-                        y1 = y1 * scale * (double)g1;
-                    }
-                    if (half) {
-                        const int l0 = sub * (HD / 2) + p0 / 2, l1 = sub * (HD / 2) + p1 / 2;
-                        const double a0 = __shfl(y0, l0, 64), b0 = __shfl(y1, l0, 64);
-                        const double a1 = __shfl(y0, l1, 64), b1 = __shfl(y1, l1, 64);
-                        const double z0 = p0 & 1 ? b0 : a0, z1 = p1 & 1 ? b1 : a1;
-                        auto turn = [&](int d, double y, double z) {
-                            if (d >= 2 * half || t >= m) return y;
-                            const double2 r = s_rot[t * half + (d < half ? d : d - half)];
-                            return d < half ? y * r.x - z * r.y : z * r.y + y * r.x;
-                        };
-                        y0 = turn(d0, y0, z0);
-                        y1 = turn(d0 + 1, y1, z1);
-                    }
-                    v[u][0] = (float)y0;
-                    v[u][1] = (float)y1;
+                    for (int j = 0; j < 4; j++) x[u][v][j] = (float)y[v][j];
                     if (hh < a.nh && t < m)
-                        *reinterpret_cast<float2 *>(a.q_out + ((size_t)(row + t) * a.nh + hh) * HD + d0) =
-                            make_float2(v[u][0], v[u][1]);
+                        *reinterpret_cast<float4 *>(a.q_out + ((size_t)(row + t) * a.nh + hh) * HD + 64 * v + d0) =
+                            make_float4(x[u][v][0], x[u][v][1], x[u][v][2], x[u][v][3]);
                 }
             }
         }
-        if (blockIdx.y * KA_WAVES + KA_WAVES <= (unsigned)a.nh) continue;   // only queries here: nothing to exchange
-
+        if (!caches) {                                               // only queries here: nothing to exchange
+            advance();
+            continue;
+        }
         const int h = hh - a.nh - (is_v ? a.nkv : 0);
         const size_t slot = cached ? ((size_t)page * a.nkv + h) * (a.c.T / 32) + pos % a.c.T / 32 : 0;
         uint8_t *dst = (uint8_t *)(is_v ? a.c.v : a.c.k) + slot * 32 * HD * EB;
-        int8_t *exps = is_v ? a.c.v_exp : a.c.k_exp;
         float inv = 1.0f, grown = 1.0f;
         bool regrow = false;
         if (F8) {
+            int8_t *exps = is_v ? a.c.v_exp : a.c.k_exp;
             int old = 0;
+            float amax = 0.0f;
             if (cached) {
                 old = exps[slot];
 #pragma unroll
-                for (int u = 0; u < STEPS; u++)
-                    if (r0 + u * TPW + sub < m)
+                for (int u = 0; u < 2; u++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            if (fabsf(v[u][e]) <= 3.402823466e38f) amax = fmaxf(amax, fabsf(v[u][e]));
+                    for (int v = 0; v < NV; v++)
 #pragma unroll
-                for (int d = 32; d >= 1; d >>= 1) amax = fmaxf(amax, __shfl_xor(amax, d, 64));
+                        for (int j = 0; j < 4; j++)      // (rows past m are zeros)
+                            if (fabsf(x[u][v][j]) <= 3.402823466e38f) amax = fmaxf(amax, fabsf(x[u][v][j]));
+                amax = wave_max_f32(amax, 0.0f);
             }
-            if (lane == 0) s_amax[w] = amax;
-            __syncthreads();
-            for (int i = 0; i < share; i++) amax = fmaxf(amax, s_amax[w - rg + i]);
+            if (share > 1) {
+                if (lane == 0) s_amax[w] = amax;
+                __syncthreads();
+                for (int i = 0; i < share; i++) amax = fmaxf(amax, s_amax[w - rg + i]);
+            }
             int e = kv_exponent(amax);
             if (off) {
                 regrow = e > old;
@@ -200,83 +300,86 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv_append(KvAppendArgs a)
                 if (regrow) grown = ldexpf(1.0f, old - e);
             }
             inv = ldexpf(1.0f, -e);
-            // (every wavefront has read `old` before the barrier)
+            // (every wavefront of the head has read `old` before the barrier)
             if (cached && lane == 0 && rg == 0 && (off == 0 || regrow)) exps[slot] = (int8_t)e;
         }
-        // the rows' codes to the tile, [row][dim]
+        // keys straight to their rows, values to the tile, [row][dim]
         if (cached) {
 #pragma unroll
-            for (int u = 0; u < STEPS; u++) {
-                const int t = r0 + u * TPW + sub;
+            for (int u = 0; u < 2; u++) {
+                const int t = r0 + 4 * u + sub;
                 if (t >= m) continue;
-                if (F8)
-                    *reinterpret_cast<uint16_t *>(tile + t * LROW + d0) = (uint16_t)kv_e4m3x2(v[u][0] * inv, v[u][1] * inv);
-                else
-                    *reinterpret_cast<kv_h2 *>(tile + t * LROW + 2 * d0) = kv_h2{(_Float16)v[u][0], (_Float16)v[u][1]};
+                uint8_t *to = is_v ? tile + t * LROW : dst + (off + t) * HD * EB;
+#pragma unroll
+                for (int v = 0; v < NV; v++) {
+                    const float *y = x[u][v];
+                    if (F8)
+                        *reinterpret_cast<uint32_t *>(to + 64 * v + d0) =
+                            kv_e4m3x2(y[0] * inv, y[1] * inv) | kv_e4m3x2(y[2] * inv, y[3] * inv) << 16;
+                    else
+                        *reinterpret_cast<uint2 *>(to + 2 * (64 * v + d0)) =
+                            make_uint2(__builtin_bit_cast(uint32_t, kv_h2{(_Float16)y[0], (_Float16)y[1]}),
+                                       __builtin_bit_cast(uint32_t, kv_h2{(_Float16)y[2], (_Float16)y[3]}));
+                }
             }
         }
         __syncthreads();
-        if (cached) {
-            auto regrown = [&](uint32_t x) {                         // four kept codes
-                const uint32_t lo = kv_e4m3x2(__builtin_amdgcn_cvt_f32_fp8(x, 0) * grown, __builtin_amdgcn_cvt_f32_fp8(x, 1) * grown);
-                const uint32_t hi = kv_e4m3x2(__builtin_amdgcn_cvt_f32_fp8(x, 2) * grown, __builtin_amdgcn_cvt_f32_fp8(x, 3) * grown);
-                return lo | hi << 16;
-            };
-            if (!is_v) {
-                constexpr int PR = HD * EB / 16;                     // pieces of a row
-                for (int i = lane + 64 * rg + (regrow ? 0 : off * PR); i < end * PR; i += 64 * share) {
-                    const int r = i / PR, p = i % PR;
-                    uint4 x;
-                    if (r >= off) {
-                        x = *reinterpret_cast<const uint4 *>(tile + (r - off) * LROW + 16 * p);
-                    } else {
-                        x = *reinterpret_cast<const uint4 *>(dst + (size_t)i * 16);
-                        x = make_uint4(regrown(x.x), regrown(x.y), regrown(x.z), regrown(x.w));
-                    }
-                    *reinterpret_cast<uint4 *>(dst + (size_t)i * 16) = x;
-                }
-            } else {
-                // 8 tokens of a dim (F16) or of two (E4M3) a piece; a piece that
-                // these rows fill in part keeps the others
-                constexpr int ND = F8 ? 2 : 1;
-                for (int i = lane + 64 * rg; i < 4 * HD / ND; i += 64 * share) {
-                    const int d = i / 4 * ND, t0 = i % 4 * 8;
-                    const bool fresh = t0 < end && t0 + 8 > off;
-                    if (!fresh && !(regrow && t0 < off)) continue;
-                    uint8_t x[16];
-                    if (t0 < off || t0 + 8 > end) {
-                        uint4 o = *reinterpret_cast<const uint4 *>(dst + (size_t)i * 16);
-                        __builtin_memcpy(x, &o, 16);
-                        if (regrow) {
-                            // what lies past these rows is no one's: only kept tokens are rewritten
-                            o = make_uint4(regrown(o.x), regrown(o.y), regrown(o.z), regrown(o.w));
-                            uint8_t n[16];
-                            __builtin_memcpy(n, &o, 16);
+        auto regrown = [&](uint32_t c) {                             // four kept codes
+            const uint32_t lo = kv_e4m3x2(__builtin_amdgcn_cvt_f32_fp8(c, 0) * grown, __builtin_amdgcn_cvt_f32_fp8(c, 1) * grown);
+            const uint32_t hi = kv_e4m3x2(__builtin_amdgcn_cvt_f32_fp8(c, 2) * grown, __builtin_amdgcn_cvt_f32_fp8(c, 3) * grown);
+            return lo | hi << 16;
+        };
+        if (cached && !is_v && regrow) {
+            for (int i = lane + 64 * rg; i < off * HD / 16; i += 64 * share) {
+                uint4 c = *reinterpret_cast<const uint4 *>(dst + (size_t)i * 16);
+                c = make_uint4(regrown(c.x), regrown(c.y), regrown(c.z), regrown(c.w));
+                *reinterpret_cast<uint4 *>(dst + (size_t)i * 16) = c;
+            }
+        }
+        if (cached && is_v) {
+            // 8 tokens of a dim (F16) or of two (E4M3) a piece; a piece that
+            // these rows fill in part keeps the others
+            constexpr int ND = F8 ? 2 : 1;
+            for (int i = lane + 64 * rg; i < 4 * HD / ND; i += 64 * share) {
+                const int d = i / 4 * ND, t0 = i % 4 * 8;
+                const bool fresh = t0 < end && t0 + 8 > off;
+                if (!fresh && !(regrow && t0 < off)) continue;
+                uint8_t y[16];
+                const uint8_t *from = tile + (t0 - off) * LROW + d * EB;
+                if (t0 >= off && t0 + 8 <= end) {
 #pragma unroll
-                            for (int j = 0; j < 16; j++)
-                                if (t0 + (j & 7) < off) x[j] = n[j];
+                    for (int j = 0; j < 8; j++) {
+                        const uint16_t x2 = *reinterpret_cast<const uint16_t *>(from + j * LROW);
+                        y[F8 ? j : 2 * j] = (uint8_t)x2;
+                        y[F8 ? 8 + j : 2 * j + 1] = (uint8_t)(x2 >> 8);
+                    }
+                } else {
+                    uint4 c = *reinterpret_cast<const uint4 *>(dst + (size_t)i * 16);
+                    __builtin_memcpy(y, &c, 16);
+                    if (regrow) {
+                        // what lies past these rows is no one's: only kept tokens are rewritten
+                        c = make_uint4(regrown(c.x), regrown(c.y), regrown(c.z), regrown(c.w));
+                        uint8_t n[16];
+                        __builtin_memcpy(n, &c, 16);
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            if (t0 + (j & 7) < off) y[j] = n[j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (t0 + j >= off && t0 + j < end) {
+                            const uint16_t x2 = *reinterpret_cast<const uint16_t *>(from + j * LROW);
+                            y[F8 ? j : 2 * j] = (uint8_t)x2;
+                            y[F8 ? 8 + j : 2 * j + 1] = (uint8_t)(x2 >> 8);
                         }
-                    }
-#pragma unroll
-                    for (int e = 0; e < ND; e++)
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            if (t0 + j >= off && t0 + j < end) {
-                                const uint8_t *from = tile + (t0 + j - off) * LROW + (d + e) * EB;
-                                if (F8) {
-                                    x[8 * e + j] = *from;
-                                } else {
-                                    x[2 * j] = from[0];
-                                    x[2 * j + 1] = from[1];
-                                }
-                            }
-                    uint4 o;
-                    __builtin_memcpy(&o, x, 16);
-                    *reinterpret_cast<uint4 *>(dst + (size_t)i * 16) = o;
                 }
+                uint4 c;
+                __builtin_memcpy(&c, y, 16);
+                *reinterpret_cast<uint4 *>(dst + (size_t)i * 16) = c;
             }
         }
         __syncthreads();                                             // the tile is the next pass's
+        advance();
     }
 }
 
@@ -286,7 +389,9 @@ hipError_t launch_kv_append(const KvAppendArgs &args, hipStream_t s)
     if (a.rd < 0 || a.rd > a.hd || a.rd % 2 || a.ks < 1) return hipErrorInvalidValue;
     a.blocks = (int32_t)kv_blocks_most(a.b.n_seqs, a.b.n_tokens);
     const int heads = a.nh + 2 * a.nkv;
-    const dim3 grid((unsigned)a.blocks + (a.rest ? 32 : 0), (heads + KA_WAVES - 1) / KA_WAVES);
+    // a head per workgroup where there are few blocks of many rows, else four
+    a.group = a.b.n_tokens >= 16 * a.b.n_seqs && (long)a.blocks * heads <= 2048 ? 1 : KA_WAVES;
+    const dim3 grid((unsigned)a.blocks + (a.rest ? 32 : 0), (heads + a.group - 1) / a.group);
     const bool f8 = a.c.type == DMOE_KV_E4M3;
     const size_t lds = (size_t)32 * (a.rd / 2) * sizeof(double2);
     switch (a.hd * (f8 ? -1 : 1)) {
