@@ -18,6 +18,8 @@
 // and lets a block's exponent grow: rows that begin inside a block keep the
 // tokens before them, whose codes are divided by 2^(e - e_old) (exact, but for
 // codes that fall under 2^-6) where e exceeds theirs.
+#include <type_traits>
+
 #include "dmoe_device.h"
 #include "dmoe_kv.h"
 
@@ -71,6 +73,16 @@ __device__ __forceinline__ double2 kv_cos_sin(double turns)
     return make_double2(q == 1 || q == 2 ? -cc : cc, q >= 2 ? -ss : ss);
 }
 
+// 1 / sqrt(x), x >= 0: two Newton steps from the hardware's estimate.
+__device__ __forceinline__ double kv_rsqrt(double x)
+{
+    double r = __builtin_amdgcn_rsq(x);
+    if (!(x > 0.0 && x < __builtin_inf())) return r;
+#pragma unroll
+    for (int i = 0; i < 2; i++) r = __builtin_fma(0.5 * r, __builtin_fma(-x * r, r, 1.0), r);
+    return r;
+}
+
 // The sum over a row's 16 lanes, in every one of them.
 __device__ __forceinline__ double kv_row_sum(double v)
 {
@@ -83,6 +95,13 @@ __device__ __forceinline__ double kv_row_sum(double v)
     KV_ROR(1);
 #undef KV_ROR
     return v;
+}
+
+// The value 8 lanes on within a row of 16.
+__device__ __forceinline__ double kv_ror8(double v)
+{
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), 0x128, 0xf, 0xf, false),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(v), 0x128, 0xf, 0xf, false));
 }
 
 // The least e with amax <= 448 * 2^e, in KV_EMIN .. KV_EMAX.  amax finite.
@@ -101,18 +120,20 @@ __device__ __forceinline__ int kv_exponent(float amax)
 // sines of the rows are formed once for all of them.  16 lanes hold a row, four
 // dims of each 64 a lane (16-byte loads; the norm's sum takes four DPP steps for
 // four rows at once).
-template <int HD, bool F8>
+// ROT: rd / 2 where it is 32 or 64 (the partners of a lane's dims are 8 lanes on,
+// or its own other vector), else -1.
+template <int HD, bool F8, int ROT>
 __global__ __launch_bounds__(KA_WAVES * 64) void k_kv_append(KvAppendArgs a)
 {
     constexpr int NV = HD / 64;                    // vectors of four dims of a lane
     constexpr int EB = F8 ? 1 : 2;
     constexpr int LROW = HD * EB + 16;             // bytes of a row in the values' tile
     __shared__ __align__(16) uint8_t s_tile[32 * LROW];
-    __shared__ __align__(16) double s_x[KA_WAVES][4 * HD];           // rows of a step, for the rotation's partners
+    __shared__ __align__(16) double s_x[KA_WAVES][ROT < 0 ? 4 * HD : 1];     // rows of a step, for the rotation's partners
     __shared__ float s_amax[KA_WAVES];
-    extern __shared__ __align__(16) double2 s_rot[];                 // [rows][rd / 2]
+    extern __shared__ __align__(16) double s_rot[];                  // cosines [rows][rd / 2], sines behind 32 rows of them
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int half = a.rd / 2, heads = a.nh + 2 * a.nkv;
+    const int half = ROT < 0 ? a.rd / 2 : ROT, heads = a.nh + 2 * a.nkv;
 
     if (blockIdx.x >= (unsigned)a.blocks) {
         // a layer's padded rows, past the last sequence's: their attention is zero
@@ -178,7 +199,8 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv_append(KvAppendArgs a)
             double2 r = kv_cos_sin((double)(pos + t) * turn), d = make_double2(1.0, 0.0);
             if (m > rows_apart) d = kv_cos_sin((double)rows_apart * turn);
             for (; t < m; t += rows_apart) {
-                s_rot[t * half + p] = r;
+                s_rot[t * half + p] = r.x;
+                s_rot[(32 + t) * half + p] = r.y;
                 r = make_double2(__builtin_fma(r.x, d.x, -(r.y * d.y)), __builtin_fma(r.x, d.y, r.y * d.x));
             }
         }
@@ -223,34 +245,60 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv_append(KvAppendArgs a)
 #pragma unroll
                         for (int j = 0; j < 4; j++) ss = __builtin_fma(y[v][j], y[v][j], ss);
                     ss = kv_row_sum(ss);
-                    const double scale = 1.0 / sqrt(ss / (double)HD + (double)a.eps);
+                    const double scale = kv_rsqrt(__builtin_fma(ss, 1.0 / HD, (double)a.eps));
 #pragma unroll
                     for (int v = 0; v < NV; v++)
 #pragma unroll
                         for (int j = 0; j < 4; j++) y[v][j] *= scale * g[v][j];
                 }
                 if (half) {
-                    double *sx = &s_x[w][sub * HD];
-                    __builtin_amdgcn_wave_barrier();
-                    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+                    // z: the other one of each dim's pair
+                    double z[NV][4];
+                    if constexpr (ROT == 32) {
 #pragma unroll
-                    for (int v = 0; v < NV; v++)
+                        for (int j = 0; j < 4; j++) z[0][j] = kv_ror8(y[0][j]);
+                    } else if constexpr (ROT == 64) {
 #pragma unroll
-                        for (int j = 0; j < 4; j++) sx[64 * v + d0 + j] = y[v][j];
-                    __builtin_amdgcn_wave_barrier();
-                    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-                    const double2 *rot = s_rot + min(t, m - 1) * half;
+                        for (int v = 0; v < NV; v++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) z[v][j] = y[NV - 1 - v][j];
+                    } else {
+                        double *sx = &s_x[w][sub * HD];
+                        __builtin_amdgcn_wave_barrier();
+                        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+#pragma unroll
+                        for (int v = 0; v < NV; v++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) sx[64 * v + d0 + j] = y[v][j];
+                        __builtin_amdgcn_wave_barrier();
+                        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+#pragma unroll
+                        for (int v = 0; v < NV; v++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                const int d = 64 * v + d0 + j;
+                                z[v][j] = sx[d < half ? d + half : d < 2 * half ? d - half : d];
+                            }
+                    }
+                    const double *rc = s_rot + min(t, m - 1) * half, *rs = rc + 32 * half;
 #pragma unroll
                     for (int v = 0; v < NV; v++) {
                         if (64 * v >= 2 * half) break;
+                        double c[4], sn[4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int d = 64 * v + d0 + j, at = min(d >= half ? d - half : d, half - 1);
+                            c[j] = rc[at];
+                            sn[j] = rs[at];
+                        }
+                        // (read whether or not the dim is rotated: a branch per dim costs more)
+                        if (ROT < 0)
+                            asm volatile("" : "+v"(c[0]), "+v"(c[1]), "+v"(c[2]), "+v"(c[3]), "+v"(sn[0]), "+v"(sn[1]), "+v"(sn[2]), "+v"(sn[3]));
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             const int d = 64 * v + d0 + j;
-                            const bool in = d < 2 * half, second = d >= half;
-                            const double2 r = rot[in ? (second ? d - half : d) : 0];
-                            const double z = sx[in ? (second ? d - half : d + half) : 0];
-                            const double to = __builtin_fma(second ? z : -z, r.y, y[v][j] * r.x);
-                            y[v][j] = in ? to : y[v][j];
+                            const double to = __builtin_fma(d >= half ? z[v][j] : -z[v][j], sn[j], y[v][j] * c[j]);
+                            y[v][j] = ROT >= 0 || d < 2 * half ? to : y[v][j];
                         }
                     }
                 }
@@ -393,14 +441,25 @@ hipError_t launch_kv_append(const KvAppendArgs &args, hipStream_t s)
     a.group = a.b.n_tokens >= 16 * a.b.n_seqs && (long)a.blocks * heads <= 2048 ? 1 : KA_WAVES;
     const dim3 grid((unsigned)a.blocks + (a.rest ? 32 : 0), (heads + a.group - 1) / a.group);
     const bool f8 = a.c.type == DMOE_KV_E4M3;
-    const size_t lds = (size_t)32 * (a.rd / 2) * sizeof(double2);
-    switch (a.hd * (f8 ? -1 : 1)) {
-    case 64: hipLaunchKernelGGL((k_kv_append<64, false>), grid, dim3(KA_WAVES * 64), lds, s, a); break;
-    case 128: hipLaunchKernelGGL((k_kv_append<128, false>), grid, dim3(KA_WAVES * 64), lds, s, a); break;
-    case -64: hipLaunchKernelGGL((k_kv_append<64, true>), grid, dim3(KA_WAVES * 64), lds, s, a); break;
-    case -128: hipLaunchKernelGGL((k_kv_append<128, true>), grid, dim3(KA_WAVES * 64), lds, s, a); break;
-    default: return hipErrorInvalidValue;
-    }
+    const size_t lds = (size_t)64 * (a.rd / 2) * sizeof(double);
+    const dim3 threads(KA_WAVES * 64);
+    auto go = [&](auto hd, auto e4m3) {
+        constexpr int HD = decltype(hd)::value;
+        constexpr bool F8 = decltype(e4m3)::value;
+        if (a.rd == 64)
+            hipLaunchKernelGGL((k_kv_append<HD, F8, 32>), grid, threads, lds, s, a);
+        else if (a.rd == 128 && HD == 128)
+            hipLaunchKernelGGL((k_kv_append<HD, F8, HD == 128 ? 64 : -1>), grid, threads, lds, s, a);
+        else
+            hipLaunchKernelGGL((k_kv_append<HD, F8, -1>), grid, threads, lds, s, a);
+    };
+    auto with = [&](auto hd) { f8 ? go(hd, std::true_type{}) : go(hd, std::false_type{}); };
+    if (a.hd == 64)
+        with(std::integral_constant<int, 64>{});
+    else if (a.hd == 128)
+        with(std::integral_constant<int, 128>{});
+    else
+        return hipErrorInvalidValue;
     return hipGetLastError();
 }
 
