@@ -28,11 +28,12 @@
 namespace dmoe {
 
 constexpr int KA_WAVES = 4;              // wavefronts of a workgroup
+constexpr int KW_WAVES = 4;              // .. of k_kv_attn_wide
 constexpr int KA_SHIFT = 4;              // probabilities are held times 2^KA_SHIFT
 constexpr int KA_SLACK = 8;              // .. and may pass that by 2^KA_SLACK before their reference is raised
 constexpr int KA_COLS = 32;              // columns of an item at most
-constexpr int KA_WHOLE = 32;             // token tiles up to which a sequence has one chunk
-constexpr int KA_CHUNK = 8;              // token tiles of a chunk at least, of longer ones
+constexpr int KA_WHOLE = 16;             // token tiles up to which a sequence has one chunk
+constexpr int KA_CHUNK = 4;              // token tiles of a chunk at least, of longer ones
 constexpr int KA_ITEMS = 512;            // items wanted of a call
 constexpr int KA_WIDE = 32768;           // columns of all kv heads from which on k_kv_attn_wide runs
 
@@ -234,34 +235,42 @@ struct KvWave {
         least = __builtin_amdgcn_readfirstlane(least);
     }
 
-    // The queries of 16 columns from col0 on as operands: put(c, hi, lo) takes
-    // chunk c.  Chunk 2 p + e of a lane holds dims 64 p + 16 g + 8 e .. + 7 (its
-    // 16 dims of a 64-dim half are one piece of an E4M3 key row).  Returns cmul.
-    template <class Put>
-    static __device__ __forceinline__ float queries(const KvAttnArgs &a, const KvSeq &q, int G, int kvh, int col0, Put &&put)
+    // The queries of 16 columns from col0 on: chunk 2 p + e of a lane holds dims
+    // 64 p + 16 g + 8 e .. + 7 (its 16 dims of a 64-dim half are one piece of an
+    // E4M3 key row).  fetch() reads them, form() makes the operands of them:
+    // put(c, hi, lo) takes chunk c; it returns cmul.
+    struct Queries {
+        float x[NC][8];
+        bool live;
+    };
+    static __device__ __forceinline__ void fetch(Queries &r, const KvAttnArgs &a, const KvSeq &q, int G, int kvh, int col0)
     {
         const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
         const int col = col0 + r16;
-        const bool live = col < q.n * G;
-        const int qi = live ? col / G : 0, hg = live ? col % G : 0;
+        r.live = col < q.n * G;
+        const int qi = r.live ? col / G : 0, hg = r.live ? col % G : 0;
         const float *src = a.q + ((size_t)(q.q0 + qi) * a.nh + (size_t)kvh * G + hg) * HD + 16 * g;
-        float x[NC][8], amax = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int j = 0; j < 8; j += 4) {
                 const float4 v = *reinterpret_cast<const float4 *>(src + 64 * (c / 2) + 8 * (c % 2) + j);
-                x[c][j] = v.x;
-                x[c][j + 1] = v.y;
-                x[c][j + 2] = v.z;
-                x[c][j + 3] = v.w;
+                r.x[c][j] = v.x;
+                r.x[c][j + 1] = v.y;
+                r.x[c][j + 2] = v.z;
+                r.x[c][j + 3] = v.w;
             }
+    }
+    template <class Put>
+    static __device__ __forceinline__ float form(Queries &r, const KvAttnArgs &a, Put &&put)
+    {
+        float amax = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                x[c][j] = live ? x[c][j] : 0.0f;
-                amax = fmaxf(amax, fabsf(x[c][j]));
+                r.x[c][j] = r.live ? r.x[c][j] : 0.0f;
+                amax = fmaxf(amax, fabsf(r.x[c][j]));
             }
         amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
         amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
@@ -277,7 +286,7 @@ struct KvWave {
             kv_h8 hi, lo;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float y = x[c][j] * mul;
+                const float y = r.x[c][j] * mul;
                 hi[j] = (_Float16)y;
                 lo[j] = (_Float16)(y - (float)hi[j]);
             }
@@ -601,6 +610,8 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
 #pragma unroll
         for (int i = 0; i < NK; i++) vr[i] = Wave::value_piece(tile, at, i);
     };
+    typename Wave::Queries queries;
+    if (w < CB) Wave::fetch(queries, a, q, G, kvh, (it.tile * CB + w) * 16);
     KvWalk<HD, F8> walk;
     walk.base = it.split * it.chunk + w;
     walk.step = KA_WAVES;
@@ -614,7 +625,7 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
     // wavefront has the same, and registers are short
     kv_h8 *s_q = reinterpret_cast<kv_h8 *>(s_o);
     if (w < CB) {
-        const float c = Wave::queries(a, q, G, kvh, (it.tile * CB + w) * 16, [&](int ch, const kv_h8 &hi, const kv_h8 &lo) {
+        const float c = Wave::form(queries, a, [&](int ch, const kv_h8 &hi, const kv_h8 &lo) {
             s_q[((w * NC + ch) * 2 + 0) * 64 + lane] = hi;
             s_q[((w * NC + ch) * 2 + 1) * 64 + lane] = lo;
         });
@@ -725,13 +736,13 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
     }
 }
 
-// Many columns of one sequence (prompts): a workgroup takes 32 KA_WAVES of
+// Many columns of one sequence (prompts): a workgroup takes 32 KW_WAVES of
 // them, each wavefront 32, over all the tokens they see.  A token tile is
 // loaded once for all four wavefronts, a quarter by each, widened to f16 and
 // left in LDS as operands (lane-contiguous: no bank conflicts); the next tile's
 // loads are in flight during its products.  The queries stay in registers.
 template <int HD, bool F8>
-__global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
+__global__ __launch_bounds__(KW_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
 {
     constexpr int CB = 2;
     typedef KvWave<HD, F8, CB> Wave;
@@ -743,7 +754,7 @@ __global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
     const int G = a.nh / a.nkv, kvh = blockIdx.x % a.nkv;
     int s, tile;
     KvSeq q;
-    const int per = 16 * CB * KA_WAVES;
+    const int per = 16 * CB * KW_WAVES;
     const int wide = a.wide;
     // the last column tiles see the most: they start first
     if (!kv_find(a.b, gridDim.x / a.nkv - 1 - blockIdx.x / a.nkv,
@@ -758,11 +769,11 @@ __global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
     uint4 r[NP];
     // wavefronts 0 and 1: keys, 2 and 3: values
     auto load = [&](size_t byte) {
-        const typename Wave::Bytes tile = Wave::at(w < KA_WAVES / 2 ? a.c.k : a.c.v, byte);
-        const uint32_t at = w < KA_WAVES / 2 ? wave.key_at() : wave.value_at();
+        const typename Wave::Bytes tile = Wave::at(w < KW_WAVES / 2 ? a.c.k : a.c.v, byte);
+        const uint32_t at = w < KW_WAVES / 2 ? wave.key_at() : wave.value_at();
 #pragma unroll
         for (int j = 0; j < NP; j++)
-            r[j] = w < KA_WAVES / 2 ? Wave::key_piece(tile, at, w * NP + j) : Wave::value_piece(tile, at, w * NP + j - NK);
+            r[j] = w < KW_WAVES / 2 ? Wave::key_piece(tile, at, w * NP + j) : Wave::value_piece(tile, at, w * NP + j - NK);
     };
     auto stage = [&](int buf) {
 #pragma unroll
@@ -781,11 +792,14 @@ __global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
     if (walk.todo) load(walk.byte());
     kv_h8 qf[CB][NC][2];
 #pragma unroll
-    for (int cb = 0; cb < CB; cb++)
-        wave.cmul[cb] = Wave::queries(a, q, G, kvh, col0 + 16 * cb, [&](int ch, const kv_h8 &hi, const kv_h8 &lo) {
+    for (int cb = 0; cb < CB; cb++) {
+        typename Wave::Queries queries;
+        Wave::fetch(queries, a, q, G, kvh, col0 + 16 * cb);
+        wave.cmul[cb] = Wave::form(queries, a, [&](int ch, const kv_h8 &hi, const kv_h8 &lo) {
             qf[cb][ch][0] = hi;
             qf[cb][ch][1] = lo;
         });
+    }
     int buf = 0;
     stage(0);
     __syncthreads();
@@ -948,11 +962,11 @@ static KvAttnPlan kv_attn_plan(const KvAttnArgs &a)
     KvAttnPlan p;
     const int64_t cols = (int64_t)a.b.n_tokens * (a.nh / a.nkv), seqs = a.b.n_seqs;
     const bool many = cols * a.nkv >= KA_WIDE;
-    p.wide = many ? (seqs == 1 ? 0 : 32 * KA_WAVES) : 0x7fffffff;
-    p.wide_items = many ? (cols / (32 * KA_WAVES) + seqs) * a.nkv : 0;
+    p.wide = many ? (seqs == 1 ? 0 : 32 * KW_WAVES) : 0x7fffffff;
+    p.wide_items = many ? (cols / (32 * KW_WAVES) + seqs) * a.nkv : 0;
     // a sequence of c columns has at most c / 32 + 1 column tiles
     int64_t tiles = cols / KA_COLS + seqs;
-    if (many) tiles = std::min(tiles, seqs * (KA_WAVES + 1));
+    if (many) tiles = std::min(tiles, seqs * (KW_WAVES + 1));
     if (p.wide == 0) tiles = 0;
     p.units = tiles * a.nkv;
     p.split = tiles > 0 && (int64_t)a.b.max_pages * (a.c.T / 32) > KA_WHOLE;
@@ -975,9 +989,8 @@ hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
     a.units = (int32_t)p.units;
     a.split = p.split;
     a.wide = p.wide;
-    const dim3 grid((unsigned)p.items), block(KA_WAVES * 64);
     if (p.wide_items) {
-        const dim3 g((unsigned)p.wide_items);
+        const dim3 g((unsigned)p.wide_items), block(KW_WAVES * 64);
         switch (a.hd * (a.c.type == DMOE_KV_E4M3 ? -1 : 1)) {
         case 64: hipLaunchKernelGGL((k_kv_attn_wide<64, false>), g, block, 0, s, a); break;
         case 128: hipLaunchKernelGGL((k_kv_attn_wide<128, false>), g, block, 0, s, a); break;
@@ -989,6 +1002,7 @@ hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
         if (e != hipSuccess) return e;
     }
     if (!p.items) return hipSuccess;
+    const dim3 grid((unsigned)p.items), block(KA_WAVES * 64);
     switch (a.hd * (a.c.type == DMOE_KV_E4M3 ? -1 : 1)) {
     case 64: hipLaunchKernelGGL((k_kv_attn<64, false>), grid, block, 0, s, a); break;
     case 128: hipLaunchKernelGGL((k_kv_attn<128, false>), grid, block, 0, s, a); break;

@@ -529,17 +529,21 @@ class Context:
                          stream=None):
         """Rows of the fused QKV projection into the paged cache, queries to
         q_out (dmoe_kv_append_device)."""
-        self._check(load().dmoe_kv_append_device(
-            self.handle, cache.ref, batch.ref, ap, _ptr(qkv), None if q_norm is None else _ptr(q_norm),
-            None if k_norm is None else _ptr(k_norm), _ptr(q_out), stream or None))
+        rc = load().dmoe_kv_append_device(
+            self.handle, cache.ref, batch.ref, ap, qkv.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
+            None if k_norm is None else k_norm.data_ptr(), q_out.data_ptr(), stream or None)
+        if rc:
+            self._check(rc)
 
     def kv_attn_device(self, cache: KvCache, batch: KvBatch, ap: AttnHParams, q, out, workspace=None, stream=None):
         """Attention of the batch's queries over the paged cache
         (dmoe_kv_attn_device); workspace: a tensor of kv_attn_workspace bytes,
         None for the context's own."""
         ws, n = self._ws(workspace)
-        self._check(load().dmoe_kv_attn_device(self.handle, cache.ref, batch.ref, ap, _ptr(q), _ptr(out), ws, n,
-                                               stream or None))
+        rc = load().dmoe_kv_attn_device(self.handle, cache.ref, batch.ref, ap, q.data_ptr(), out.data_ptr(), ws, n,
+                                        stream or None)
+        if rc:
+            self._check(rc)
 
     def kv_attn_workspace(self, cache: KvCache, batch: KvBatch, ap: AttnHParams) -> int:
         n = load().dmoe_kv_attn_workspace(self.handle, cache.ref, batch.ref, ap)
