@@ -41,20 +41,39 @@ __device__ __forceinline__ int kv_wave_scan(int v)
     return v;
 }
 
+// Sequence base + lane of 64, and which rows are its: `top` is the largest first
+// row met so far (0 before the first 64).  In a table that decreases, a sequence
+// whose rows could be an earlier one's has none, so that the rows of all of them
+// are disjoint and the counts that follow from n_tokens hold for any table.
+__device__ __forceinline__ KvSeq kv_seqs(const KvBatch &b, int base, int &top)
+{
+    const int s = base + (threadIdx.x & 63);
+    KvSeq q{0, 0, 0};
+    if (s < b.n_seqs) q = kv_seq(b, s);
+    int v = max(top, (unsigned)q.q0 <= (unsigned)b.n_tokens ? q.q0 : 0);
+#define KV_DPP(ctrl, rows) v = max(v, __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, false))
+    KV_DPP(0x111, 0xf);                  // the running maximum, as in kv_wave_scan
+    KV_DPP(0x112, 0xf);
+    KV_DPP(0x114, 0xf);
+    KV_DPP(0x118, 0xf);
+    KV_DPP(0x142, 0xa);
+    KV_DPP(0x143, 0xc);
+#undef KV_DPP
+    top = __builtin_amdgcn_readlane(v, 63);
+    if (v > q.q0) q.n = 0;
+    return q;
+}
+
 // Item `item` of a list that holds count(seq) items of each sequence in turn:
 // its sequence (and the item's index within it), found by one wavefront in
 // steps of 64 sequences; false past the list's end.
 template <class Count>
 __device__ __forceinline__ bool kv_find(const KvBatch &b, int item, Count &&count, int &seq, KvSeq &info, int &index)
 {
-    const int lane = threadIdx.x & 63;
+    int top = 0;
     for (int base = 0; base < b.n_seqs; base += 64) {
-        KvSeq q{0, 0, 0};
-        int c = 0;
-        if (base + lane < b.n_seqs) {
-            q = kv_seq(b, base + lane);
-            c = count(q);
-        }
+        const KvSeq q = kv_seqs(b, base, top);
+        const int c = count(q);
         const int end = kv_wave_scan(c);
         const uint64_t past = __ballot(end > item);
         if (past) {

@@ -102,7 +102,7 @@ __device__ __forceinline__ int kv_blocks_of_tile(int cols) { return cols <= 16 ?
 
 __device__ __forceinline__ int kv_token_tiles(const KvAttnArgs &a, const KvSeq &q)
 {
-    return (kv_cached(q.len, a.c.T, a.b.max_pages) + 31) / 32;
+    return q.n ? (kv_cached(q.len, a.c.T, a.b.max_pages) + 31) / 32 : 0;
 }
 
 __device__ __forceinline__ int kv_col_tiles(const KvAttnArgs &a, const KvSeq &q, int G)
@@ -136,16 +136,12 @@ __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, Kv
         const float items = fmaxf((float)KA_ITEMS - 0.5f * u * (float)a.nkv, 0.25f * (float)KA_ITEMS);
         C = max(KA_CHUNK, (int)(w * (float)a.nkv / items) + 1);
     }
+    int top = 0;
     for (int base = 0; base < a.b.n_seqs; base += 64) {
-        KvSeq q{0, 0, 0};
-        int tiles = 0, ks = 1;
-        if (base + lane < a.b.n_seqs) {
-            q = kv_seq(a.b, base + lane);
-            tiles = kv_col_tiles(a, q, G);
-            // (a sequence without tokens still has its rows to zero)
-            const int length = kv_token_tiles(a, q);
-            if (length > KA_WHOLE) ks = (length + C - 1) / C;
-        }
+        const KvSeq q = kv_seqs(a.b, base, top);
+        const int tiles = kv_col_tiles(a, q, G), length = kv_token_tiles(a, q);
+        // (one without tokens still has its rows to zero)
+        const int ks = length > KA_WHOLE ? (length + C - 1) / C : 1;
         const int count = tiles * ks * a.nkv, end = kv_wave_scan(count), before = kv_wave_scan(tiles) - tiles;
         const uint64_t past = __ballot(end > item);
         if (past) {
@@ -960,7 +956,8 @@ struct KvAttnPlan {
 static KvAttnPlan kv_attn_plan(const KvAttnArgs &a)
 {
     KvAttnPlan p;
-    const int64_t cols = (int64_t)a.b.n_tokens * (a.nh / a.nkv), seqs = a.b.n_seqs;
+    const int64_t cols = (int64_t)a.b.n_tokens * (a.nh / a.nkv);
+    const int64_t seqs = std::min(a.b.n_seqs, a.b.n_tokens);       // .. with rows
     const bool many = cols * a.nkv >= KA_WIDE;
     p.wide = many ? (seqs == 1 ? 0 : 32 * KW_WAVES) : 0x7fffffff;
     p.wide_items = many ? (cols / (32 * KW_WAVES) + seqs) * a.nkv : 0;

@@ -282,7 +282,8 @@ typedef struct dmoe_kv_cache {
  * (-1, say) and a token past the table hold nothing: an append skips them, the
  * attention does not see them.  A sequence whose numbers contradict each other
  * (rows outside 0 .. n_tokens, kv_len below its number of rows or above 2^30)
- * is treated as one without rows.  The three tables are read on the stream: a captured call
+ * is treated as one without rows, and so is one that starts below an earlier
+ * entry of q_start.  The three tables are read on the stream: a captured call
  * sees what they hold at each replay. */
 typedef struct dmoe_kv_batch {
     int32_t n_seqs;

@@ -169,3 +169,18 @@ def test_pages_and_masks(ask):
     want = [1, 6, 32, 40, 40, 32, 1 << 31, big, 40]
     want[6] = min(big, 64 * (1 << 25))
     assert [int(x) for x in ask([("sees", list(c)) for c in cases])] == want
+
+
+def test_structs_lie_as_in_c(tmp_path):
+    """The ctypes mirrors have the size and offsets of include/dmoe.h's."""
+    import ctypes
+    from dmoe import _abi
+    pairs = (("dmoe_kv_cache", _abi.KvCacheStruct), ("dmoe_kv_batch", _abi.KvBatchStruct))
+    src = tmp_path / "layout.c"
+    body = "".join(f'printf("%zu\\n", sizeof({n}));' + "".join(f'printf("%zu\\n", offsetof({n}, {f}));' for f, _ in c._fields_)
+                   for n, c in pairs)
+    src.write_text(f'#include <stdio.h>\n#include <stddef.h>\n#include "{ROOT}/include/dmoe.h"\nint main(void) {{ {body} return 0; }}\n')
+    subprocess.run(["gcc", "-o", str(tmp_path / "layout"), str(src)], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True, check=True).stdout.split()]
+    want = [x for _, c in pairs for x in [ctypes.sizeof(c)] + [getattr(c, f).offset for f, _ in c._fields_]]
+    assert got == want
