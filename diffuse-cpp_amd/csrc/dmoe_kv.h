@@ -27,18 +27,33 @@ __device__ __forceinline__ KvSeq kv_seq(const KvBatch &b, int s)
     return kv_seq_of(b.q_start[s], b.q_start[s + 1], b.kv_len[s], b.n_tokens);
 }
 
-// Inclusive prefix sum over the 64 lanes, by DPP.
-__device__ __forceinline__ int kv_wave_scan(int v)
+// Inclusive scan over the 64 lanes, by DPP (0 is neutral to `op`).
+template <class T, class Op>
+__device__ __forceinline__ T kv_wave_scan(T v, Op &&op)
 {
-#define KV_DPP(ctrl, rows) __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, false)
-    v += KV_DPP(0x111, 0xf);             // row_shr 1, 2, 4, 8
-    v += KV_DPP(0x112, 0xf);
-    v += KV_DPP(0x114, 0xf);
-    v += KV_DPP(0x118, 0xf);
-    v += KV_DPP(0x142, 0xa);             // lane 15 of rows 0 and 2 to rows 1 and 3
-    v += KV_DPP(0x143, 0xc);             // lane 31 to rows 2 and 3
+#define KV_DPP(ctrl, rows) \
+    v = op(v, __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, rows, 0xf, false)))
+    KV_DPP(0x111, 0xf);                  // row_shr 1, 2, 4, 8
+    KV_DPP(0x112, 0xf);
+    KV_DPP(0x114, 0xf);
+    KV_DPP(0x118, 0xf);
+    KV_DPP(0x142, 0xa);                  // lane 15 of rows 0 and 2 to rows 1 and 3
+    KV_DPP(0x143, 0xc);                  // lane 31 to rows 2 and 3
 #undef KV_DPP
     return v;
+}
+
+template <class T>
+__device__ __forceinline__ T kv_wave_scan(T v)
+{
+    return kv_wave_scan(v, [](T x, T y) { return x + y; });
+}
+
+// A scan's last value, which is the whole wavefront's.
+template <class T>
+__device__ __forceinline__ T kv_wave_last(T v)
+{
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // Sequence base + lane of 64, and which rows are its: `top` is the largest first
@@ -50,16 +65,9 @@ __device__ __forceinline__ KvSeq kv_seqs(const KvBatch &b, int base, int &top)
     const int s = base + (threadIdx.x & 63);
     KvSeq q{0, 0, 0};
     if (s < b.n_seqs) q = kv_seq(b, s);
-    int v = max(top, (unsigned)q.q0 <= (unsigned)b.n_tokens ? q.q0 : 0);
-#define KV_DPP(ctrl, rows) v = max(v, __builtin_amdgcn_update_dpp(0, v, ctrl, rows, 0xf, false))
-    KV_DPP(0x111, 0xf);                  // the running maximum, as in kv_wave_scan
-    KV_DPP(0x112, 0xf);
-    KV_DPP(0x114, 0xf);
-    KV_DPP(0x118, 0xf);
-    KV_DPP(0x142, 0xa);
-    KV_DPP(0x143, 0xc);
-#undef KV_DPP
-    top = __builtin_amdgcn_readlane(v, 63);
+    const int first = max(top, (unsigned)q.q0 <= (unsigned)b.n_tokens ? q.q0 : 0);
+    const int v = kv_wave_scan(first, [](int x, int y) { return max(x, y); });
+    top = kv_wave_last(v);
     if (v > q.q0) q.n = 0;
     return q;
 }
@@ -85,7 +93,7 @@ __device__ __forceinline__ bool kv_find(const KvBatch &b, int item, Count &&coun
             index = item - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(c, l));
             return true;
         }
-        item -= __builtin_amdgcn_readlane(end, 63);
+        item -= kv_wave_last(end);
     }
     return false;
 }

@@ -54,8 +54,8 @@ KV_HD int64_t kv_blocks_most(int n_seqs, int n_tokens)
 // the table.
 KV_HD int kv_entry_of(int pos, int page_tokens, int max_pages)
 {
-    const int i = pos / page_tokens;
-    return i < max_pages ? i : -1;
+    const uint32_t i = (uint32_t)pos / (uint32_t)page_tokens;
+    return i < (uint32_t)max_pages ? (int)i : -1;
 }
 
 // The page of an entry, or -1 for one that is no page of the cache.
@@ -75,8 +75,9 @@ KV_HD int kv_cached(int len, int page_tokens, int max_pages)
 KV_HD int kv_visible(int pos, int cached, int block)
 {
     if (block <= 0) return cached;
-    const int64_t end = ((int64_t)pos / block + 1) * block;
-    return end < cached ? (int)end : cached;
+    // (below 2^32: pos is below 2^30, and so is pos / block * block)
+    const uint32_t end = ((uint32_t)pos / (uint32_t)block + 1) * (uint32_t)block;
+    return end < (uint32_t)cached ? (int)end : cached;
 }
 
 // ---------------------------------------------------------------------------

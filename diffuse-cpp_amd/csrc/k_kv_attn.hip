@@ -83,7 +83,8 @@ __device__ __forceinline__ kv_h8 kv_cut(const kv_h8 &v, int g, int lim)
 // one column tile of one kv head over one chunk of token tiles.  The chunk
 // length is common to all sequences, so that ragged ones spread over the chip
 // like one: the total of (column tile, token tile) pairs over the items wanted,
-// at least KA_CHUNK.  A sequence's chunks are then made equally long.
+// at least KA_CHUNK.  A sequence's chunks are then made equally long, and one of
+// up to KA_WHOLE token tiles is not cut.
 //
 // A sequence's items lie kv heads first, then chunks, then column tiles: what
 // reads the same keys is a multiple of the kv heads apart, and as workgroups go
@@ -115,53 +116,76 @@ __device__ __forceinline__ int kv_col_tiles(const KvAttnArgs &a, const KvSeq &q,
 // sequences at a time.
 __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, KvItem &it)
 {
-    const int lane = threadIdx.x & 63;
-    int C = 0x7fffffff, units = 0;
-    if (a.split) {
-        float w = 0.0f, u = 0.0f;        // exact enough: a length, not an index
-        for (int base = 0; base < a.b.n_seqs; base += 64)
-            if (base + lane < a.b.n_seqs) {
-                const KvSeq q = kv_seq(a.b, base + lane);
-                const float tiles = (float)kv_col_tiles(a, q, G);
-                u += tiles;
-                w += tiles * (float)kv_token_tiles(a, q);
-            }
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) {
-            w += __shfl_xor(w, d, 64);
-            u += __shfl_xor(u, d, 64);
-        }
-        // a column tile's last chunk is half empty on average: so many items
-        // fewer are shared out, that all start in one round
-        const float items = fmaxf((float)KA_ITEMS - 0.5f * u * (float)a.nkv, 0.25f * (float)KA_ITEMS);
-        C = max(KA_CHUNK, (int)(w * (float)a.nkv / items) + 1);
-    }
     int top = 0;
-    for (int base = 0; base < a.b.n_seqs; base += 64) {
-        const KvSeq q = kv_seqs(a.b, base, top);
-        const int tiles = kv_col_tiles(a, q, G), length = kv_token_tiles(a, q);
-        // (one without tokens still has its rows to zero)
-        const int ks = length > KA_WHOLE ? (length + C - 1) / C : 1;
-        const int count = tiles * ks * a.nkv, end = kv_wave_scan(count), before = kv_wave_scan(tiles) - tiles;
-        const uint64_t past = __ballot(end > item);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            auto at = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            it.s = base + l;
-            it.q = KvSeq{at(q.q0), at(q.n), at(q.len)};
-            it.cb = kv_blocks_of_tile(it.q.n * G);
-            it.ks = at(ks);
-            it.chunk = (kv_token_tiles(a, it.q) + it.ks - 1) / it.ks;
-            const int i = item - (at(end) - at(count));
-            it.kvh = i % a.nkv;
-            it.split = i / a.nkv % it.ks;
-            it.tile = i / a.nkv / it.ks;
-            it.unit = (units + at(before) + it.tile) * a.nkv + it.kvh;
-            return true;
+    KvSeq q = kv_seqs(a.b, 0, top);
+    // f(first sequence) with q a lane's of 64 sequences, until it returns true;
+    // of up to 64 they are read once
+    auto each = [&](auto &&f) {
+        if (a.b.n_seqs <= 64) return f(0);
+        top = 0;
+        for (int base = 0; base < a.b.n_seqs; base += 64) {
+            q = kv_seqs(a.b, base, top);
+            if (f(base)) return true;
         }
-        item -= __builtin_amdgcn_readlane(end, 63);
-        units += __builtin_amdgcn_readlane(before + tiles, 63);
+        return false;
+    };
+    int C = 0x7fffffff;
+    if (a.split) {
+        // items of a kv head that the short sequences have, column tiles and
+        // pairs of tiles of the others (exact enough: lengths, not indexes)
+        float few = 0.0f, many = 0.0f, work = 0.0f;
+        each([&](int) {
+            const float tiles = (float)kv_col_tiles(a, q, G);
+            const int length = kv_token_tiles(a, q);
+            few += length > KA_WHOLE ? 0.0f : tiles;
+            many += length > KA_WHOLE ? tiles : 0.0f;
+            work += length > KA_WHOLE ? tiles * (float)length : 0.0f;
+            return false;
+        });
+        few = kv_wave_last(kv_wave_scan(few));
+        many = kv_wave_last(kv_wave_scan(many));
+        work = kv_wave_last(kv_wave_scan(work));
+        // What all can start at once is shared out; a column tile's last chunk
+        // is half empty on average, and where that is not enough the count
+        // says by how much.
+        const float all = (float)KA_ITEMS / (float)a.nkv, least = 0.25f * all;
+        C = max(KA_CHUNK, (int)(work / fmaxf(all - few - 0.5f * many, least)) + 1);
+        float count = 0.0f;
+        each([&](int) {
+            const int length = kv_token_tiles(a, q);
+            if (length > KA_WHOLE) count += (float)(kv_col_tiles(a, q, G) * (int)((uint32_t)(length + C - 1) / (uint32_t)C));
+            return false;
+        });
+        count = kv_wave_last(kv_wave_scan(count));
+        if (count > all - few) C = (int)((float)C * fmaxf(1.0f, count / fmaxf(all - few, least))) + 1;
     }
+    int units = 0;
+    if (each([&](int base) {
+            const int tiles = kv_col_tiles(a, q, G), length = kv_token_tiles(a, q);
+            // (one without tokens still has its rows to zero)
+            const int ks = length > KA_WHOLE ? (int)((uint32_t)(length + C - 1) / (uint32_t)C) : 1;
+            const int count = tiles * ks * a.nkv, end = kv_wave_scan(count), before = kv_wave_scan(tiles) - tiles;
+            const uint64_t past = __ballot(end > item);
+            if (!past) {
+                item -= kv_wave_last(end);
+                units += kv_wave_last(before + tiles);
+                return false;
+            }
+            const int l = __builtin_ctzll(past);
+            auto at = [&](int v) { return (uint32_t)__builtin_amdgcn_readlane(v, l); };
+            const uint32_t n = at(ks), i = (uint32_t)item - (at(end) - at(count));
+            it.s = base + l;
+            it.q = KvSeq{(int)at(q.q0), (int)at(q.n), (int)at(q.len)};
+            it.cb = kv_blocks_of_tile(it.q.n * G);
+            it.ks = (int)n;
+            it.chunk = (int)((at(length) + n - 1) / n);
+            it.kvh = (int)(i % (uint32_t)a.nkv);
+            it.split = (int)(i / (uint32_t)a.nkv % n);
+            it.tile = (int)(i / (uint32_t)a.nkv / n);
+            it.unit = (units + (int)at(before) + it.tile) * a.nkv + it.kvh;
+            return true;
+        }))
+        return true;
     it.unit = units * a.nkv;             // how many there are
     return false;
 }
@@ -214,7 +238,7 @@ struct KvWave {
         for (int cb = 0; cb < CB; cb++) {
             const int col = col0 + 16 * cb + r16;
             const bool live = col < q.n * G;
-            vis[cb] = live ? kv_visible(q.len - q.n + col / G, cached, a.block) : 0;
+            vis[cb] = live ? kv_visible(q.len - q.n + (int)((uint32_t)col / (uint32_t)G), cached, a.block) : 0;
             last = max(last, vis[cb]);
             if (live) least = min(least, vis[cb]);
             m[cb] = -__builtin_inff();
@@ -244,8 +268,8 @@ struct KvWave {
         const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
         const int col = col0 + r16;
         r.live = col < q.n * G;
-        const int qi = r.live ? col / G : 0, hg = r.live ? col % G : 0;
-        const float *src = a.q + ((size_t)(q.q0 + qi) * a.nh + (size_t)kvh * G + hg) * HD + 16 * g;
+        const uint32_t qi = r.live ? (uint32_t)col / (uint32_t)G : 0, hg = r.live ? (uint32_t)col % (uint32_t)G : 0;
+        const float *src = a.q + ((size_t)(q.q0 + (int)qi) * a.nh + (size_t)kvh * G + hg) * HD + 16 * g;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -545,7 +569,7 @@ struct KvWalk {
         const int tt = base + step * (int)(threadIdx.x & 63);
         int page = -1;
         if (tt < end) page = kv_page(a.b, a.c, s, 32 * tt);
-        const size_t slot = ((size_t)max(page, 0) * a.nkv + kvh) * (a.c.T / 32) + tt % (a.c.T / 32);
+        const size_t slot = ((size_t)max(page, 0) * a.nkv + kvh) * (a.c.T / 32) + (uint32_t)tt % (uint32_t)(a.c.T / 32);
         const size_t byte = slot * 32 * HD * (F8 ? 1 : 2);
         blo = (uint32_t)byte;
         bhi = (uint32_t)(byte >> 32);
