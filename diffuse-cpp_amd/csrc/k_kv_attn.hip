@@ -36,6 +36,7 @@ constexpr int KA_WHOLE = 16;             // token tiles up to which a sequence h
 constexpr int KA_CHUNK = 4;              // token tiles of a chunk at least, of longer ones
 constexpr int KA_ITEMS = 512;            // items wanted of a call
 constexpr int KA_WIDE = 32768;           // columns of all kv heads from which on k_kv_attn_wide runs
+constexpr int KA_LONG = 64;              // token tiles up to which it takes sequences with fewer columns than that
 
 // one 16-byte piece of cache as f16: F16 8 values, E4M3 16
 template <bool F8>
@@ -95,7 +96,8 @@ struct KvItem {
     int s, kvh, tile, split;             // sequence, kv head, column tile, chunk
     int cb;                              // 16-column blocks of a tile
     int ks, chunk;                       // chunks of the sequence, token tiles of each
-    int unit;                            // column tile and kv head, counted over the call
+    int part, unit;                      // of a sequence with several chunks: among such items, and among such
+                                         // (column tile, kv head)s
 };
 
 // 16-column blocks of a tile of a sequence with `cols` columns
@@ -106,10 +108,17 @@ __device__ __forceinline__ int kv_token_tiles(const KvAttnArgs &a, const KvSeq &
     return q.n ? (kv_cached(q.len, a.c.T, a.b.max_pages) + 31) / 32 : 0;
 }
 
+// Whether k_kv_attn_wide takes a sequence of a call in which it runs.
+__device__ __forceinline__ bool kv_is_wide(const KvAttnArgs &a, const KvSeq &q, int G)
+{
+    const int cols = q.n * G;
+    return cols > a.wide && (a.wide == 0 || cols * a.nkv >= KA_WIDE || kv_token_tiles(a, q) <= KA_LONG);
+}
+
 __device__ __forceinline__ int kv_col_tiles(const KvAttnArgs &a, const KvSeq &q, int G)
 {
     const int cols = q.n * G, per = 16 * kv_blocks_of_tile(cols);
-    return cols > a.wide ? 0 : (cols + per - 1) / per;
+    return kv_is_wide(a, q, G) ? 0 : (cols + per - 1) / per;
 }
 
 // Item `item` of the call, or false past the last.  One wavefront, 64
@@ -159,16 +168,18 @@ __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, Kv
         count = kv_wave_last(kv_wave_scan(count));
         if (count > all - few) C = (int)((float)C * fmaxf(1.0f, count / fmaxf(all - few, least))) + 1;
     }
-    int units = 0;
+    int parts = 0, units = 0;
     if (each([&](int base) {
             const int tiles = kv_col_tiles(a, q, G), length = kv_token_tiles(a, q);
             // (one without tokens still has its rows to zero)
             const int ks = length > KA_WHOLE ? (int)((uint32_t)(length + C - 1) / (uint32_t)C) : 1;
-            const int count = tiles * ks * a.nkv, end = kv_wave_scan(count), before = kv_wave_scan(tiles) - tiles;
+            const int count = tiles * ks * a.nkv, part = ks > 1 ? tiles * ks : 0, unit = ks > 1 ? tiles : 0;
+            const int end = kv_wave_scan(count), parts_end = kv_wave_scan(part), units_end = kv_wave_scan(unit);
             const uint64_t past = __ballot(end > item);
             if (!past) {
                 item -= kv_wave_last(end);
-                units += kv_wave_last(before + tiles);
+                parts += kv_wave_last(parts_end);
+                units += kv_wave_last(units_end);
                 return false;
             }
             const int l = __builtin_ctzll(past);
@@ -182,7 +193,8 @@ __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, Kv
             it.kvh = (int)(i % (uint32_t)a.nkv);
             it.split = (int)(i / (uint32_t)a.nkv % n);
             it.tile = (int)(i / (uint32_t)a.nkv / n);
-            it.unit = (units + (int)at(before) + it.tile) * a.nkv + it.kvh;
+            it.part = (parts + (int)(at(parts_end) - at(part))) * a.nkv + (int)i;
+            it.unit = (units + (int)(at(units_end) - at(unit)) + it.tile) * a.nkv + it.kvh;
             return true;
         }))
         return true;
@@ -190,17 +202,20 @@ __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, Kv
     return false;
 }
 
-// The workspace of a call whose sequences can have several chunks: for each
-// unit what the join has to know, then per item its columns' sums
-// [KA_COLS][HD] and their (m, l).
+// The workspace of a call whose sequences can have several chunks: how many
+// units the join has, for each what it has to know, then per item of them its
+// columns' sums [KA_COLS][HD] and their (m, l).  A unit of several chunks is
+// longer than a chunk, whose length is at least the work over KA_ITEMS: there
+// are at most KA_ITEMS units and 2 KA_ITEMS items of this kind, however many
+// columns the call has.
 struct KvDesc {
-    int32_t ks, item, tile, kvh, q0, cols, cb, pad;      // item: the unit's first
+    int32_t ks, part, tile, kvh, q0, cols, cb, pad;      // part: the unit's first
 };
 
 template <int HD>
-__device__ __forceinline__ float *kv_part(const KvAttnArgs &a, int item)
+__device__ __forceinline__ float *kv_part(const KvAttnArgs &a, int part)
 {
-    return (float *)((KvDesc *)a.ws + a.units) + (size_t)item * KA_COLS * (HD + 2);
+    return (float *)((KvDesc *)a.ws + 1 + a.units) + (size_t)part * KA_COLS * (HD + 2);
 }
 
 // ---------------------------------------------------------------------------
@@ -749,7 +764,7 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
             *reinterpret_cast<float4 *>(a.out + ((size_t)(q.q0 + cc / G) * a.nh + (size_t)kvh * G + cc % G) * HD + d) =
                 make_float4(O.x * inv, O.y * inv, O.z * inv, O.w * inv);
         } else {
-            float *part = kv_part<HD>(a, blockIdx.x);
+            float *part = kv_part<HD>(a, it.part);
             *reinterpret_cast<float4 *>(part + c * HD + d) = O;
             if (d == 0) *reinterpret_cast<float2 *>(part + KA_COLS * HD + 2 * c) = make_float2(M, L);
         }
@@ -775,10 +790,9 @@ __global__ __launch_bounds__(KW_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
     int s, tile;
     KvSeq q;
     const int per = 16 * CB * KW_WAVES;
-    const int wide = a.wide;
     // the last column tiles see the most: they start first
     if (!kv_find(a.b, gridDim.x / a.nkv - 1 - blockIdx.x / a.nkv,
-                 [=](const KvSeq &r) { return r.n * G > wide ? (r.n * G + per - 1) / per : 0; }, s, q, tile))
+                 [&](const KvSeq &r) { return kv_is_wide(a, r, G) ? (r.n * G + per - 1) / per : 0; }, s, q, tile))
         return;
     const int col0 = tile * per + w * 16 * CB;
     Wave wave;
@@ -903,15 +917,13 @@ __global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn(KvAttnArgs a)
     const int G = a.nh / a.nkv;
     KvItem it;
     if (!kv_item(a, G, blockIdx.x, it)) {
-        // at least as many items as units stay empty (the launch's bound): each
-        // item past the last marks one of those
-        const int u = it.unit + (gridDim.x - 1 - blockIdx.x);
-        if (a.split && threadIdx.x == 0 && u < a.units) ((KvDesc *)a.ws)[u].ks = 0;
+        // (the launch's bound on the items is never reached)
+        if (a.split && threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) *(int32_t *)a.ws = it.unit;
         return;
     }
-    if (a.split && it.split == 0 && threadIdx.x == 0)
-        ((KvDesc *)a.ws)[it.unit] = KvDesc{it.ks, (int)blockIdx.x, it.tile, it.kvh, it.q.q0,
-                                           min(16 * it.cb, it.q.n * G - it.tile * 16 * it.cb), it.cb, 0};
+    if (it.ks > 1 && it.split == 0 && threadIdx.x == 0)
+        ((KvDesc *)a.ws)[1 + it.unit] = KvDesc{it.ks, it.part, it.tile, it.kvh, it.q.q0,
+                                               min(16 * it.cb, it.q.n * G - it.tile * 16 * it.cb), it.cb, 0};
     if (it.cb == 1)
         kv_attend<HD, F8, 1>(a, it, G, s_o, s_m, s_l);
     else
@@ -926,9 +938,10 @@ __global__ __launch_bounds__(THREADS) void k_kv_join(KvAttnArgs a)
     constexpr int ND = HD / 4, PARTS = THREADS / (COLS * ND);
     __shared__ __align__(16) float4 s_o[PARTS][COLS][ND];
     __shared__ float s_m[PARTS][COLS], s_l[PARTS][COLS];
-    const KvDesc d = ((const KvDesc *)a.ws)[blockIdx.x];
+    const int units = *(const int32_t *)a.ws;
+    const KvDesc d = ((const KvDesc *)a.ws)[1 + blockIdx.x];
     const int c0 = blockIdx.y * COLS;
-    if (d.ks <= 1 || c0 >= d.cols) return;
+    if ((int)blockIdx.x >= units || c0 >= d.cols) return;
     const int e = threadIdx.x % ND, ci = threadIdx.x / ND % COLS, part = threadIdx.x / (ND * COLS);
     const int c = min(c0 + ci, d.cols - 1);
     const float inf = __builtin_inff();
@@ -936,7 +949,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_join(KvAttnArgs a)
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
     for (int j = part; j < d.ks; j += PARTS) {
-        const float *p = kv_part<HD>(a, d.item + j * a.nkv);
+        const float *p = kv_part<HD>(a, d.part + j * a.nkv);
         const float2 ml = *reinterpret_cast<const float2 *>(p + KA_COLS * HD + 2 * c);
         const float4 x = *reinterpret_cast<const float4 *>(p + c * HD + 4 * e);
         const float mn = fmaxf(m, ml.x);
@@ -972,8 +985,9 @@ __global__ __launch_bounds__(THREADS) void k_kv_join(KvAttnArgs a)
 // What the launches take: the items at most, and whether any sequence can have
 // several chunks (from the page table's width: the lengths are on the GPU).
 struct KvAttnPlan {
-    int64_t items, units, wide_items;    // items and units of k_kv_attn at most, items of k_kv_attn_wide
-    int32_t wide;                        // columns from which on a sequence is k_kv_attn_wide's
+    int64_t items, wide_items;           // of k_kv_attn and k_kv_attn_wide at most
+    int64_t units, parts;                // what the workspace holds
+    int32_t wide;                        // columns above which a sequence can be k_kv_attn_wide's
     bool split;
 };
 
@@ -985,21 +999,22 @@ static KvAttnPlan kv_attn_plan(const KvAttnArgs &a)
     const bool many = cols * a.nkv >= KA_WIDE;
     p.wide = many ? (seqs == 1 ? 0 : 32 * KW_WAVES) : 0x7fffffff;
     p.wide_items = many ? (cols / (32 * KW_WAVES) + seqs) * a.nkv : 0;
-    // a sequence of c columns has at most c / 32 + 1 column tiles
-    int64_t tiles = cols / KA_COLS + seqs;
-    if (many) tiles = std::min(tiles, seqs * (KW_WAVES + 1));
-    if (p.wide == 0) tiles = 0;
-    p.units = tiles * a.nkv;
+    // a sequence of c columns has at most c / 32 + 1 column tiles, and one that
+    // is not k_kv_attn_wide's has not more than these columns
+    const int64_t most = std::max<int64_t>(KA_WIDE / a.nkv, 32 * KW_WAVES);
+    const int64_t tiles = p.wide == 0 ? 0 : std::min(cols / KA_COLS + seqs, many ? seqs * (most / KA_COLS + 1) : cols + seqs);
     p.split = tiles > 0 && (int64_t)a.b.max_pages * (a.c.T / 32) > KA_WHOLE;
     // chunks: less than one more per unit than its share of those wanted
-    p.items = p.units + (p.split ? KA_ITEMS : 0);
+    p.items = tiles * a.nkv + (p.split ? KA_ITEMS + 1 : 0);
+    p.units = std::min<int64_t>(tiles * a.nkv, KA_ITEMS);
+    p.parts = std::min<int64_t>(p.items, 2 * KA_ITEMS);
     return p;
 }
 
 size_t kv_attn_ws_bytes(const KvAttnArgs &a)
 {
     const KvAttnPlan p = kv_attn_plan(a);
-    return p.split ? (size_t)p.units * sizeof(KvDesc) + (size_t)p.items * KA_COLS * (a.hd + 2) * 4 : 256;
+    return p.split ? (size_t)(1 + p.units) * sizeof(KvDesc) + (size_t)p.parts * KA_COLS * (a.hd + 2) * 4 : 256;
 }
 
 hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
