@@ -35,7 +35,7 @@ constexpr int KA_COLS = 32;              // columns of an item at most
 constexpr int KA_WHOLE = 16;             // token tiles up to which a sequence has one chunk
 constexpr int KA_CHUNK = 4;              // token tiles of a chunk at least, of longer ones
 constexpr int KA_ITEMS = 512;            // items wanted of a call
-constexpr int KA_WIDE = 32768;           // columns of all kv heads from which on k_kv_attn_wide runs
+constexpr int KA_WIDE = 57344;           // columns of all kv heads from which on k_kv_attn_wide runs
 constexpr int KA_LONG = 64;              // token tiles up to which it takes sequences with fewer columns than that
 
 // one 16-byte piece of cache as f16: F16 8 values, E4M3 16
@@ -140,25 +140,28 @@ __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, Kv
     };
     int C = 0x7fffffff;
     if (a.split) {
-        // items of a kv head that the short sequences have, column tiles and
-        // pairs of tiles of the others (exact enough: lengths, not indexes)
-        float few = 0.0f, many = 0.0f, work = 0.0f;
+        // column tiles of the sequences that are not cut and of the others, and
+        // their pairs of tiles (exact enough: lengths, not indexes)
+        float few = 0.0f, many = 0.0f, rest = 0.0f, work = 0.0f;
         each([&](int) {
             const float tiles = (float)kv_col_tiles(a, q, G);
             const int length = kv_token_tiles(a, q);
-            few += length > KA_WHOLE ? 0.0f : tiles;
-            many += length > KA_WHOLE ? tiles : 0.0f;
-            work += length > KA_WHOLE ? tiles * (float)length : 0.0f;
+            (length > KA_WHOLE ? many : few) += tiles;
+            (length > KA_WHOLE ? work : rest) += tiles * (float)length;
             return false;
         });
         few = kv_wave_last(kv_wave_scan(few));
         many = kv_wave_last(kv_wave_scan(many));
+        rest = kv_wave_last(kv_wave_scan(rest));
         work = kv_wave_last(kv_wave_scan(work));
         // What all can start at once is shared out; a column tile's last chunk
         // is half empty on average, and where that is not enough the count
-        // says by how much.
-        const float all = (float)KA_ITEMS / (float)a.nkv, least = 0.25f * all;
-        C = max(KA_CHUNK, (int)(work / fmaxf(all - few - 0.5f * many, least)) + 1);
+        // says by how much.  If that would make a chunk twice as long as an
+        // item's share of all the work, the items start one after the other
+        // anyhow, and the share it is.
+        const float all = (float)KA_ITEMS / (float)a.nkv, share = (work + rest) / all + 1.0f;
+        float c = work / fmaxf(all - few - 0.5f * many, 0.25f * all) + 1.0f;
+        C = max(KA_CHUNK, (int)c);
         float count = 0.0f;
         each([&](int) {
             const int length = kv_token_tiles(a, q);
@@ -166,7 +169,8 @@ __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, Kv
             return false;
         });
         count = kv_wave_last(kv_wave_scan(count));
-        if (count > all - few) C = (int)((float)C * fmaxf(1.0f, count / fmaxf(all - few, least))) + 1;
+        if (count > all - few) c = fmaxf((float)C, c * count / fmaxf(all - few, 0.25f * all) + 1.0f);
+        C = max(KA_CHUNK, (int)(c > 2.0f * share ? share : c));
     }
     int parts = 0, units = 0;
     if (each([&](int base) {

@@ -66,9 +66,10 @@ def _check(batch, cache, q, block, got):
 
 # rows of 8 heads to a kv head: 16 of them are 128 columns
 GROUPS = {
-    "one": [(0, 1030)], "after": [(90, 1025)], "long": [(2500, 1100)],
-    "beside": [(5, 3), (0, 0), (2100, 513), (700, 1), (31, 16), (0, 17), (63, 70), (1, 450), (900, 33)],
+    "one": [(0, 1800)], "after": [(90, 1795)], "long": [(2500, 1830)],
+    "beside": [(5, 3), (0, 0), (2100, 513), (700, 1), (31, 16), (0, 17), (63, 70), (1, 1150), (900, 33)],
     "padded": [(3000, 40)],                          # fewer rows than the buffers hold
+    "many": [(i * 397 % 1700, i % 6) for i in range(150)],
 }
 
 
@@ -82,7 +83,7 @@ def _q(batch, nh, hd, seed):
 def test_prompts(ctx, kvtype, group, block):
     nh, nkv, hd, T = 32, 4, 128, 64
     print(f"case: attn {kvtype} prompt {group}, block {block}", flush=True)
-    batch = R.Batch(GROUPS[group], T, seed=1, extra=1000 if group == "padded" else 3)
+    batch = R.Batch(GROUPS[group], T, seed=1, extra=1800 if group == "padded" else 3)
     cache = R.Cache(kvtype, batch.n_pages, nkv, hd, T, seed=2)
     _poison(batch, cache)
     q = _q(batch, nh, hd, 3)
@@ -94,7 +95,7 @@ def test_prompts(ctx, kvtype, group, block):
 def test_prompts_of_other_shapes(ctx, kvtype, shape):
     nh, nkv, hd, T = shape
     print(f"case: attn {kvtype} prompt {shape}", flush=True)
-    n = -(-32768 // nh)
+    n = -(-57344 // nh)
     for seqs in ([(77, n)], [(0, n - n // 3), (5, 1), (130, n // 3)]):
         batch = R.Batch(seqs, T, seed=4, extra=1)
         cache = R.Cache(kvtype, batch.n_pages, nkv, hd, T, seed=5)
@@ -109,7 +110,7 @@ def test_prompts_with_pages_that_are_none(ctx, kvtype):
     """Holes, a sequence without a page, the first 64 token tiles of one without."""
     nh, nkv, hd, T = 32, 4, 64, 32
     print(f"case: attn {kvtype} prompts, pages that are none", flush=True)
-    for seqs in ([(2200, 1030)], [(40, 300), (2200, 800), (2, 9)]):
+    for seqs in ([(2200, 1800)], [(40, 300), (2200, 1800), (2, 9)]):
         batch = R.Batch(seqs, T, seed=7)
         long = len(seqs) // 2
         if long:
@@ -132,7 +133,7 @@ def test_prompts_what_is_not_seen_has_no_part(ctx, kvtype, block):
     """NaN and infinities at positions that some rows of a tile see."""
     nh, nkv, hd, T = 32, 2, 64, 32
     print(f"case: attn {kvtype} prompt, block {block}, NaN in masked places", flush=True)
-    batch = R.Batch([(20, 1024), (0, 64)], T, seed=10)
+    batch = R.Batch([(20, 1792), (0, 64)], T, seed=10)
     cache = R.Cache(kvtype, batch.n_pages, nkv, hd, T, seed=11)
     q = _q(batch, nh, hd, 12)
     clean = _run(ctx, batch, cache, q, block)
@@ -201,7 +202,7 @@ def test_pages_looked_up_several_times(ctx, kvtype):
     _check(batch, cache, q, 1, _run(ctx, batch, cache, q, 1))
 
 
-@pytest.mark.parametrize("n", [2, 1024])
+@pytest.mark.parametrize("n", [2, 1800])
 def test_rows_of_an_earlier_sequence(ctx, n):
     """Tables that decrease: sequences that start below an earlier entry of
     q_start have no rows, in the append and in the attention; the others are as
