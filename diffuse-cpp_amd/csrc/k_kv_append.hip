@@ -206,6 +206,19 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv_append(KvAppendArgs a)
         }
     }
     __syncthreads();
+    // A lane's dims and rows are the same in every pass, and where the partners'
+    // distance is known its dims' angles are those of four pairs
+    double c[2][4], sn[2][4];
+    if (ROT >= 0) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const double *rc = s_rot + min(r0 + 4 * u + sub, m - 1) * half + d0 % half + j;
+                c[u][j] = rc[0];
+                sn[u][j] = rc[32 * half];
+            }
+    }
 
     for (int hb = head0; hb < head1; hb += KA_WAVES / share) {
         const int hh = hb + w / share;
@@ -284,20 +297,20 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv_append(KvAppendArgs a)
 #pragma unroll
                     for (int v = 0; v < NV; v++) {
                         if (64 * v >= 2 * half) break;
-                        double c[4], sn[4];
+                        if (ROT < 0) {
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const int d = 64 * v + d0 + j, at = min(d >= half ? d - half : d, half - 1);
-                            c[j] = rc[at];
-                            sn[j] = rs[at];
+                            for (int j = 0; j < 4; j++) {
+                                const int d = 64 * v + d0 + j, at = min(d >= half ? d - half : d, half - 1);
+                                c[u][j] = rc[at];
+                                sn[u][j] = rs[at];
+                            }
+                            // (read whether or not the dim is rotated: a branch per dim costs more)
+                            asm volatile("" : "+v"(c[u][0]), "+v"(c[u][1]), "+v"(c[u][2]), "+v"(c[u][3]), "+v"(sn[u][0]), "+v"(sn[u][1]), "+v"(sn[u][2]), "+v"(sn[u][3]));
                         }
-                        // (read whether or not the dim is rotated: a branch per dim costs more)
-                        if (ROT < 0)
-                            asm volatile("" : "+v"(c[0]), "+v"(c[1]), "+v"(c[2]), "+v"(c[3]), "+v"(sn[0]), "+v"(sn[1]), "+v"(sn[2]), "+v"(sn[3]));
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             const int d = 64 * v + d0 + j;
-                            const double to = __builtin_fma(d >= half ? z[v][j] : -z[v][j], sn[j], y[v][j] * c[j]);
+                            const double to = __builtin_fma(d >= half ? z[v][j] : -z[v][j], sn[u][j], y[v][j] * c[u][j]);
                             y[v][j] = ROT >= 0 || d < 2 * half ? to : y[v][j];
                         }
                     }
