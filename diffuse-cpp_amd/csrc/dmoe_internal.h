@@ -256,7 +256,7 @@ struct KvAppendArgs {
     const float *q_norm, *k_norm;
     float *q_out;                        // [n_tokens][nh][hd]
     float *rest;                         // when given: rows of [n_tokens][nh][hd] past the last sequence's to zero
-    int32_t blocks, group;               // set by the launch
+    int32_t blocks, group, zeros;        // set by the launch
 };
 hipError_t launch_kv_append(const KvAppendArgs &a, hipStream_t s);
 struct KvAttnArgs {

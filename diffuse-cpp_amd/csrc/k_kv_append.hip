@@ -120,6 +120,11 @@ __device__ __forceinline__ int kv_exponent(float amax)
 // sines of the rows are formed once for all of them.  16 lanes hold a row, four
 // dims of each 64 a lane (16-byte loads; the norm's sum takes four DPP steps for
 // four rows at once).
+// Bound by its bytes: 4001 rows of 32 + 2 * 4 heads of 128 with an E4M3 cache,
+// 152 MB, take 32.9 us, 4.6 TB/s of the 5.15 that a large copy reaches; without
+// the norm and the rotation it is no faster.  What that took: a block's head
+// groups next to each other in the grid (36.1 us, before that 40) and query
+// stores past the caches (37.3, before that 42.2).
 // ROT: rd / 2 where it is 32 or 64 (the partners of a lane's dims are 8 lanes on,
 // or its own other vector), else -1.
 template <int HD, bool F8, int ROT>
@@ -135,19 +140,21 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv_append(KvAppendArgs a)
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int half = ROT < 0 ? a.rd / 2 : ROT, heads = a.nh + 2 * a.nkv;
 
-    if (blockIdx.x >= (unsigned)a.blocks) {
+    // a block's head groups one after the other: what runs at a time covers whole rows
+    const uint32_t groups = gridDim.x / (uint32_t)(a.blocks + a.zeros), item = blockIdx.x / groups, hg = blockIdx.x % groups;
+    if (item >= (uint32_t)a.blocks) {
         // a layer's padded rows, past the last sequence's: their attention is zero
         const int64_t first = (int64_t)min(max(a.b.q_start[a.b.n_seqs], 0), a.b.n_tokens) * a.nh * HD;
         const int64_t n = (int64_t)a.b.n_tokens * a.nh * HD - first;
-        const int64_t step = (int64_t)(gridDim.x - a.blocks) * gridDim.y * KA_WAVES * 64 * 4;
-        const int64_t i0 = ((int64_t)(blockIdx.x - a.blocks) * gridDim.y + blockIdx.y) * KA_WAVES * 64 + threadIdx.x;
+        const int64_t step = (int64_t)a.zeros * groups * KA_WAVES * 64 * 4;
+        const int64_t i0 = (int64_t)(blockIdx.x - a.blocks * groups) * KA_WAVES * 64 + threadIdx.x;
         for (int64_t i = 4 * i0; i < n; i += step)
             *reinterpret_cast<float4 *>(a.rest + first + i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         return;
     }
     int s, blk;
     KvSeq q;
-    if (!kv_find(a.b, blockIdx.x, [](const KvSeq &r) { return kv_blocks(r); }, s, q, blk)) return;
+    if (!kv_find(a.b, (int)item, [](const KvSeq &r) { return kv_blocks(r); }, s, q, blk)) return;
     const int pos_q = q.len - q.n;                                   // the first row's position
     const int pos = max(pos_q, (pos_q / 32 + blk) * 32);             // this block's first row
     const int off = pos % 32;
@@ -161,7 +168,7 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv_append(KvAppendArgs a)
     uint8_t *tile = s_tile + (w / share) * share * 8 * LROW;         // rows of this wavefront's head
     const int sub = lane >> 4, d0 = 4 * (lane & 15);                 // row of a step; dims d0 + 64 v ..
     const size_t row_floats = (size_t)heads * HD;
-    const int head0 = blockIdx.y * a.group, head1 = min(head0 + a.group, heads);
+    const int head0 = (int)hg * a.group, head1 = min(head0 + a.group, heads);
     const bool rotates = head0 < a.nh + a.nkv, caches = head1 > a.nh;
 
     float x[2][NV][4], next[2][NV][4];
@@ -320,8 +327,9 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv_append(KvAppendArgs a)
 #pragma unroll
                     for (int j = 0; j < 4; j++) x[u][v][j] = (float)y[v][j];
                     if (hh < a.nh && t < m)
-                        *reinterpret_cast<float4 *>(a.q_out + ((size_t)(row + t) * a.nh + hh) * HD + 64 * v + d0) =
-                            make_float4(x[u][v][0], x[u][v][1], x[u][v][2], x[u][v][3]);
+                        // (past the caches: written once, and read by other CUs if at all)
+                        __builtin_nontemporal_store(kv_f4{x[u][v][0], x[u][v][1], x[u][v][2], x[u][v][3]},
+                                                    reinterpret_cast<kv_f4 *>(a.q_out + ((size_t)(row + t) * a.nh + hh) * HD + 64 * v + d0));
                 }
             }
         }
@@ -450,9 +458,14 @@ hipError_t launch_kv_append(const KvAppendArgs &args, hipStream_t s)
     if (a.rd < 0 || a.rd > a.hd || a.rd % 2 || a.ks < 1) return hipErrorInvalidValue;
     a.blocks = (int32_t)kv_blocks_most(a.b.n_seqs, a.b.n_tokens);
     const int heads = a.nh + 2 * a.nkv;
-    // a head per workgroup where there are few blocks of many rows, else four
-    a.group = a.b.n_tokens >= 16 * a.b.n_seqs && (long)a.blocks * heads <= 2048 ? 1 : KA_WAVES;
-    const dim3 grid((unsigned)a.blocks + (a.rest ? 32 : 0), (heads + a.group - 1) / a.group);
+    // Heads of a workgroup.  Few rows a sequence: four, which its wavefronts take
+    // at once (61 rows of 61 sequences 7.3 us, two heads 9.9).  Many: one where the
+    // chip has places for all (16 blocks of 32 rows 8.0, two 10.0), else two, the
+    // second's loads in flight during the first (4001 rows 32.9, one 38.9, four
+    // 36.1, eight 40.9).
+    a.group = a.b.n_tokens < 16 * a.b.n_seqs ? KA_WAVES : (long)a.blocks * heads <= 2048 ? 1 : 2;
+    a.zeros = a.rest ? 32 : 0;
+    const dim3 grid((unsigned)((a.blocks + a.zeros) * ((heads + a.group - 1) / a.group)));
     const bool f8 = a.c.type == DMOE_KV_E4M3;
     const size_t lds = (size_t)64 * (a.rd / 2) * sizeof(double);
     const dim3 threads(KA_WAVES * 64);
