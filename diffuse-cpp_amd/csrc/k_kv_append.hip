@@ -122,9 +122,9 @@ __device__ __forceinline__ int kv_exponent(float amax)
 // four rows at once).
 // Bound by its bytes: 4001 rows of 32 + 2 * 4 heads of 128 with an E4M3 cache,
 // 152 MB, take 32.9 us, 4.6 TB/s of the 5.15 that a large copy reaches; without
-// the norm and the rotation it is no faster.  What that took: a block's head
-// groups next to each other in the grid (36.1 us, before that 40) and query
-// stores past the caches (37.3, before that 42.2).
+// the norm and the rotation it is no faster.  What that took (at four heads a
+// workgroup, 42.2 us without either): a block's head groups next to each other in
+// the grid, 40.8, query stores past the caches, 37.3, both, 36.1.
 // ROT: rd / 2 where it is 32 or 64 (the partners of a lane's dims are 8 lanes on,
 // or its own other vector), else -1.
 template <int HD, bool F8, int ROT>

@@ -936,15 +936,15 @@ __global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn(KvAttnArgs a)
 
 // Joins the chunks of a unit: a workgroup takes COLS of its columns, its
 // threads four dims of a column and every PARTS-th chunk.
-template <int HD, int COLS, int THREADS>
+template <int HD, int DIMS, int COLS, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_kv_join(KvAttnArgs a)
 {
-    constexpr int ND = HD / 4, PARTS = THREADS / (COLS * ND);
+    constexpr int ND = DIMS / 4, PARTS = THREADS / (COLS * ND);
     __shared__ __align__(16) float4 s_o[PARTS][COLS][ND];
     __shared__ float s_m[PARTS][COLS], s_l[PARTS][COLS];
     const int units = *(const int32_t *)a.ws;
     const KvDesc d = ((const KvDesc *)a.ws)[1 + blockIdx.x];
-    const int c0 = blockIdx.y * COLS;
+    const int c0 = (int)blockIdx.y / (HD / DIMS) * COLS, d0 = (int)blockIdx.y % (HD / DIMS) * DIMS;
     if ((int)blockIdx.x >= units || c0 >= d.cols) return;
     const int e = threadIdx.x % ND, ci = threadIdx.x / ND % COLS, part = threadIdx.x / (ND * COLS);
     const int c = min(c0 + ci, d.cols - 1);
@@ -955,7 +955,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_join(KvAttnArgs a)
     for (int j = part; j < d.ks; j += PARTS) {
         const float *p = kv_part<HD>(a, d.part + j * a.nkv);
         const float2 ml = *reinterpret_cast<const float2 *>(p + KA_COLS * HD + 2 * c);
-        const float4 x = *reinterpret_cast<const float4 *>(p + c * HD + 4 * e);
+        const float4 x = *reinterpret_cast<const float4 *>(p + c * HD + d0 + 4 * e);
         const float mn = fmaxf(m, ml.x);
         const float f = m == -inf ? 0.0f : __builtin_amdgcn_exp2f(m - mn), h = ml.x == -inf ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
         m = mn;
@@ -982,7 +982,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_join(KvAttnArgs a)
     }
     const int G = a.nh / a.nkv, col = d.tile * 16 * d.cb + c;
     const float inv = m == -inf ? 0.0f : 1.0f / l;
-    *reinterpret_cast<float4 *>(a.out + ((size_t)(d.q0 + col / G) * a.nh + (size_t)d.kvh * G + col % G) * HD + 4 * e) =
+    *reinterpret_cast<float4 *>(a.out + ((size_t)(d.q0 + col / G) * a.nh + (size_t)d.kvh * G + col % G) * HD + d0 + 4 * e) =
         make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
@@ -1057,15 +1057,16 @@ hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
     // time, as most of a launch that has a workgroup for every column a unit
     // could have only starts and ends.
     const bool deep = p.units <= 32;
-    const dim3 join((unsigned)p.units, deep ? KA_COLS : KA_COLS / 4), threads(deep ? 512 : 256);
+    const unsigned cols = deep ? KA_COLS * (a.hd / 64) : KA_COLS / 4;
+    const dim3 join((unsigned)p.units, cols), threads(deep ? 512 : 256);
     if (a.hd == 64 && deep)
-        hipLaunchKernelGGL((k_kv_join<64, 1, 512>), join, threads, 0, s, a);
+        hipLaunchKernelGGL((k_kv_join<64, 64, 1, 512>), join, threads, 0, s, a);
     else if (a.hd == 64)
-        hipLaunchKernelGGL((k_kv_join<64, 4, 256>), join, threads, 0, s, a);
+        hipLaunchKernelGGL((k_kv_join<64, 64, 4, 256>), join, threads, 0, s, a);
     else if (deep)
-        hipLaunchKernelGGL((k_kv_join<128, 1, 512>), join, threads, 0, s, a);
+        hipLaunchKernelGGL((k_kv_join<128, 64, 1, 512>), join, threads, 0, s, a);
     else
-        hipLaunchKernelGGL((k_kv_join<128, 4, 256>), join, threads, 0, s, a);
+        hipLaunchKernelGGL((k_kv_join<128, 128, 4, 256>), join, threads, 0, s, a);
     return hipGetLastError();
 }
 
