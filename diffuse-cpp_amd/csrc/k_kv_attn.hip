@@ -15,7 +15,7 @@
 //
 // E4M3: key and value of token j are code * 2^ke and code * 2^ve of its block.
 // 2^ke goes into the scores' factor; ve is added to the exponent of the
-// probabilities (p' = 2^(s + ve - m'), at most 1 by the choice of m'), and the
+// probabilities (p' = 2^(s + ve - m'), at most 2^KA_SLACK), and the
 // sum takes p' 2^-ve: no operand is rescaled.  With exponents within 100 of
 // each other no p' that counts in the sum underflows.
 #include <algorithm>
@@ -27,16 +27,34 @@
 
 namespace dmoe {
 
+// Times: 32 query and 4 kv heads of 128, kernel and join, in us.
 constexpr int KA_WAVES = 4;              // wavefronts of a workgroup
 constexpr int KW_WAVES = 4;              // .. of k_kv_attn_wide
 constexpr int KA_SHIFT = 4;              // probabilities are held times 2^KA_SHIFT
-constexpr int KA_SLACK = 8;              // .. and may pass that by 2^KA_SLACK before their reference is raised
+// .. and may pass that by 2^KA_SLACK (f16 reaches 2^16) before their column's
+// reference is raised: a block of 32 rows on 16,384 tokens 29.2, with 0 34.8
+constexpr int KA_SLACK = 8;
 constexpr int KA_COLS = 32;              // columns of an item at most
-constexpr int KA_WHOLE = 16;             // token tiles up to which a sequence has one chunk
-constexpr int KA_CHUNK = 4;              // token tiles of a chunk at least, of longer ones
-constexpr int KA_ITEMS = 512;            // items wanted of a call
-constexpr int KA_WIDE = 57344;           // columns of all kv heads from which on k_kv_attn_wide runs
-constexpr int KA_LONG = 64;              // token tiles up to which it takes sequences with fewer columns than that
+// A sequence of up to KA_WHOLE token tiles has one chunk, the others chunks of
+// KA_CHUNK tiles at least: one row on 512 F16 tokens takes 12.4 whole, cut 9.3 and
+// 3.6 for the join; on 700 14.8 whole, 9.5 + 3.4 in chunks of four tiles, 11.3 +
+// 3.8 of eight.  A CU takes in about 50 GB/s, so that more of them pay early.
+constexpr int KA_WHOLE = 16;
+constexpr int KA_CHUNK = 4;
+// Items wanted of a call, two workgroups for each of 256 CUs.  (256 of eight
+// wavefronts: 131,072 tokens of one row the same, 48 sequences of one row 61, not 48.)
+constexpr int KA_ITEMS = 512;
+// Columns of all kv heads from which on k_kv_attn_wide runs, a workgroup for 128
+// of them: it reads a token tile once for them, where k_kv_attn does it for 32, but
+// needs a workgroup on most CUs twice.  A prompt of 2000 rows 109 against 128 in
+// F16, 102 against 99 in E4M3, on 4000 cached tokens 312 against 348; of 1024 rows
+// 60 against 55 and 54 against 43.
+constexpr int KA_WIDE = 57344;
+// Beside others it takes sequences with fewer columns than that if they have up to
+// KA_LONG token tiles, for it does not cut them: 31 blocks of 32 rows on 1024
+// tokens and one on 32,768 take 131 (F16) and 106 (E4M3), with 16 tiles 390 and 332,
+// with no limit 1495 and 1433.
+constexpr int KA_LONG = 64;
 
 // one 16-byte piece of cache as f16: F16 8 values, E4M3 16
 template <bool F8>
@@ -100,7 +118,8 @@ struct KvItem {
                                          // (column tile, kv head)s
 };
 
-// 16-column blocks of a tile of a sequence with `cols` columns
+// 16-column blocks of a tile of a sequence with `cols` columns.  (Two for few
+// columns too: one row on 700 tokens 11.0, not 9.5, on 131,072 33.0, not 30.3.)
 __device__ __forceinline__ int kv_blocks_of_tile(int cols) { return cols <= 16 ? 1 : 2; }
 
 __device__ __forceinline__ int kv_token_tiles(const KvAttnArgs &a, const KvSeq &q)
@@ -617,7 +636,13 @@ struct KvWalk {
 };
 
 // One item's columns, 16 CB of them: the workgroup's wavefronts take its token
-// tiles in turn and join their results in LDS.  A tile's keys and values go
+// tiles in turn and join their results in LDS.  Few rows are bound by the bytes:
+// 48 of 8190 E4M3 tokens each, 229 MB, 48.2 us and 4.8 of the join (4.75 TB/s of
+// the 5.15 that a large copy reaches), one of 131,072, 134 MB, 30.3 and 5.3.  Blocks
+// by the products: 32 rows on 16,384 tokens, 17.2 GFLOP with both halves, 29.2 and
+// 4.6, of them 7.7 until the first scores stand (work list, page, tile: three
+// loads one after the other), 15 for the tiles (14.4 at the rate of a large
+// library product) and 2.7 to join the wavefronts.  A tile's keys and values go
 // straight from global memory to the registers that hold them as operands; the
 // next tile's keys are loaded once a tile's scores stand, its values once its
 // sums do, so that loads are always in flight and no second set of registers
@@ -780,6 +805,9 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
 // loaded once for all four wavefronts, a quarter by each, widened to f16 and
 // left in LDS as operands (lane-contiguous: no bank conflicts); the next tile's
 // loads are in flight during its products.  The queries stay in registers.
+// Bound by the products: 2000 rows on 4001 cached tokens and themselves, 328 GFLOP
+// with both halves, in 276 to 284 us, 1,160 to 1,190 TFLOP/s, which is what a large
+// f16 product of the library reaches here.
 template <int HD, bool F8>
 __global__ __launch_bounds__(KW_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
 {
@@ -1052,11 +1080,12 @@ hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.split) return e;
-    // Few units have many chunks each (KA_ITEMS in all): a workgroup per column
-    // then, 16 or 32 chunks at a time; else one per four columns, two or four at a
-    // time, as most of a launch that has a workgroup for every column a unit
-    // could have only starts and ends.
-    const bool deep = p.units <= 32;
+    // Few units can have many chunks each (KA_ITEMS in all): 32 of them at a time
+    // then, a workgroup per column and 64 dims (4 units of 128 chunks 5.3 us, the
+    // other form 11.2).  Else a workgroup per four columns: most of the launch,
+    // which has places for every column a unit could have, only starts and ends
+    // (32 units of 16 chunks 4.6 against 8.7, 4 units of 6 chunks 3.4 against 4.0).
+    const bool deep = p.units <= 32 && (int64_t)a.b.max_pages * (a.c.T / 32) > 16 * KA_CHUNK;
     const unsigned cols = deep ? KA_COLS * (a.hd / 64) : KA_COLS / 4;
     const dim3 join((unsigned)p.units, cols), threads(deep ? 512 : 256);
     if (a.hd == 64 && deep)
