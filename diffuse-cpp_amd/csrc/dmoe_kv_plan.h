@@ -28,6 +28,8 @@ struct KvSeq {
     int q0, n, len;
 };
 constexpr int KV_TOKENS_MOST = 1 << 30;
+// Rows and sequences of a call, times n_head + 2 n_head_kv.
+constexpr int64_t KV_ROWS_MOST = 1 << 27, KV_SEQS_MOST = 1 << 24;
 
 KV_HD KvSeq kv_seq_of(int start, int end, int len, int n_tokens)
 {
@@ -101,6 +103,24 @@ inline bool kv_overlap(const void *a, size_t na, const void *b, size_t nb)
     return x < y + nb && y < x + na;
 }
 
+inline size_t kv_cache_blocks(const dmoe_kv_cache &kv)
+{
+    return (size_t)kv.n_pages * kv.n_head_kv * (kv.page_tokens / DMOE_KV_BLOCK);
+}
+
+inline size_t kv_cache_bytes(const dmoe_kv_cache &kv)
+{
+    return kv_cache_blocks(kv) * DMOE_KV_BLOCK * kv.head_dim * (kv.type == DMOE_KV_E4M3 ? 1 : 2);
+}
+
+// Whether a buffer shares memory with a cache (checked before).
+inline bool kv_in_cache(const dmoe_kv_cache &kv, const void *p, size_t n)
+{
+    const size_t bytes = kv_cache_bytes(kv), blocks = kv.type == DMOE_KV_E4M3 ? kv_cache_blocks(kv) : 0;
+    return kv_overlap(p, n, kv.k, bytes) || kv_overlap(p, n, kv.v, bytes) ||
+           (blocks && (kv_overlap(p, n, kv.k_exp, blocks) || kv_overlap(p, n, kv.v_exp, blocks)));
+}
+
 // A cache, a batch and the attention's sizes; `pointers`: those too.
 inline int kv_check(KvRefusal &r, const dmoe_kv_cache *kv, const dmoe_kv_batch *b, const dmoe_attn_hparams *ap,
                     bool pointers)
@@ -123,9 +143,10 @@ inline int kv_check(KvRefusal &r, const dmoe_kv_cache *kv, const dmoe_kv_batch *
     if (b->n_seqs <= 0 || b->n_tokens <= 0 || b->max_pages <= 0)
         return r.set(DMOE_ERR_INVALID_ARG, "kv: n_seqs = %d, n_tokens = %d, max_pages = %d must be positive", b->n_seqs,
                      b->n_tokens, b->max_pages);
-    // grids and the indexes of (row, head) pairs are 32 bits wide
-    if ((int64_t)b->n_tokens * (ap->n_head + 2 * (int64_t)ap->n_head_kv) > INT32_MAX / 2 || b->n_seqs > (1 << 20) ||
-        ap->n_head > 65535 || ap->n_head_kv > 32767)
+    // the indexes of (row, head) pairs are 32 bits wide, and a launch has less
+    // than 2^24 workgroups of 256 threads
+    const int64_t heads = ap->n_head + 2 * (int64_t)ap->n_head_kv;
+    if (heads > KV_SEQS_MOST || b->n_tokens * heads > KV_ROWS_MOST || b->n_seqs * heads > KV_SEQS_MOST || b->n_seqs > (1 << 20))
         return r.set(DMOE_ERR_SHAPE, "kv: %d rows of %d + 2 * %d heads, %d sequences are too many", b->n_tokens,
                      ap->n_head, ap->n_head_kv, b->n_seqs);
     if (!pointers) return DMOE_OK;
@@ -134,8 +155,7 @@ inline int kv_check(KvRefusal &r, const dmoe_kv_cache *kv, const dmoe_kv_batch *
         return r.set(DMOE_ERR_INVALID_ARG, "kv: a pointer of the cache is NULL");
     if ((uintptr_t)kv->k % 16 || (uintptr_t)kv->v % 16)
         return r.set(DMOE_ERR_INVALID_ARG, "kv: k and v must be 16-byte aligned");
-    const size_t blocks = (size_t)kv->n_pages * kv->n_head_kv * (kv->page_tokens / DMOE_KV_BLOCK);
-    const size_t bytes = blocks * DMOE_KV_BLOCK * kv->head_dim * (f8 ? 1 : 2);
+    const size_t blocks = kv_cache_blocks(*kv), bytes = kv_cache_bytes(*kv);
     if (kv_overlap(kv->k, bytes, kv->v, bytes) || (f8 && kv_overlap(kv->k_exp, blocks, kv->v_exp, blocks)))
         return r.set(DMOE_ERR_INVALID_ARG, "kv: keys and values overlap");
     if (!b->q_start || !b->kv_len || !b->pages) return r.set(DMOE_ERR_INVALID_ARG, "kv: a table of the batch is NULL");
@@ -166,6 +186,9 @@ inline int kv_check_append(KvRefusal &r, const dmoe_kv_cache *kv, const dmoe_kv_
     const size_t head = (size_t)b->n_tokens * ap->head_dim * 4;
     if (kv_overlap(qkv, head * ((size_t)ap->n_head + 2 * (size_t)ap->n_head_kv), q_out, head * ap->n_head))
         return r.set(DMOE_ERR_INVALID_ARG, "kv_append: qkv and q_out overlap");
+    if (kv_in_cache(*kv, qkv, head * ((size_t)ap->n_head + 2 * (size_t)ap->n_head_kv)) ||
+        kv_in_cache(*kv, q_out, head * ap->n_head))
+        return r.set(DMOE_ERR_INVALID_ARG, "kv_append: qkv or q_out overlaps the cache");
     return DMOE_OK;
 }
 
@@ -178,6 +201,7 @@ inline int kv_check_attn(KvRefusal &r, const dmoe_kv_cache *kv, const dmoe_kv_ba
         return r.set(DMOE_ERR_INVALID_ARG, "kv_attn: q and out must be 16-byte aligned");
     const size_t bytes = (size_t)b->n_tokens * ap->n_head * ap->head_dim * 4;
     if (kv_overlap(q, bytes, out, bytes)) return r.set(DMOE_ERR_INVALID_ARG, "kv_attn: q and out overlap");
+    if (kv_in_cache(*kv, out, bytes)) return r.set(DMOE_ERR_INVALID_ARG, "kv_attn: out overlaps the cache");
     return DMOE_OK;
 }
 
@@ -192,6 +216,8 @@ inline int kv_check_layer(KvRefusal &r, const dmoe_kv_cache *kv, const dmoe_kv_b
     if ((h_out != h && kv_overlap(h, bytes, h_out, bytes)) ||
         (moe_in && (kv_overlap(moe_in, bytes, h, bytes) || kv_overlap(moe_in, bytes, h_out, bytes))))
         return r.set(DMOE_ERR_INVALID_ARG, "attn_cached: h, h_out and moe_in overlap");
+    if (kv_in_cache(*kv, h, bytes) || kv_in_cache(*kv, h_out, bytes) || (moe_in && kv_in_cache(*kv, moe_in, bytes)))
+        return r.set(DMOE_ERR_INVALID_ARG, "attn_cached: h, h_out or moe_in overlaps the cache");
     return DMOE_OK;
 }
 

@@ -5,6 +5,10 @@ torch tensors on the context's GPU, which the caller keeps alive.
     batch = dmoe.KvBatch(q_start, kv_len, pages, n_tokens)       # int32 tensors
     ctx.kv_append_device(cache, batch, ap, qkv, q, q_norm, k_norm, stream=s)
     ctx.kv_attn_device(cache, batch, ap, q, out, stream=s)
+
+The cache's and the batch's tensors are checked here, once; a call's own buffers
+are contiguous float32 tensors of the size that the header states, as in the
+other device calls.
 """
 from __future__ import annotations
 
@@ -31,6 +35,12 @@ def _whole(t, dtype, name):
     return t
 
 
+def _one_gpu(*tensors):
+    devices = {str(t.device) for t in tensors if t is not None}
+    if len(devices) != 1 or not tensors[0].is_cuda:
+        raise ValueError(f"the tensors are on {sorted(devices)}, not on one GPU")
+
+
 class KvCache:
     """k [n_pages, n_head_kv, page_tokens, head_dim]; v [n_pages, n_head_kv,
     page_tokens / 32, head_dim, 32] (float16) or [.., head_dim / 2, 4, 2, 8]
@@ -55,6 +65,7 @@ class KvCache:
                 if e is None or tuple(e.shape) != blocks:
                     raise ValueError(f"{name}: shape {blocks} is needed")
                 _whole(e, "torch.int8", name)
+        _one_gpu(k, v, *([k_exp, v_exp] if f8 else []))
         self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
         self.struct = KvCacheStruct(KV_E4M3 if f8 else KV_F16, H, D, T, P, k.data_ptr(), v.data_ptr(),
                                     k_exp.data_ptr() if f8 else None, v_exp.data_ptr() if f8 else None)
@@ -83,6 +94,7 @@ class KvBatch:
             raise ValueError(f"q_start {tuple(q_start.shape)}, kv_len {tuple(kv_len.shape)}, pages {tuple(pages.shape)}")
         for name, t in (("q_start", q_start), ("kv_len", kv_len), ("pages", pages)):
             _whole(t, "torch.int32", name)
+        _one_gpu(q_start, kv_len, pages)
         self.q_start, self.kv_len, self.pages, self.n_tokens = q_start, kv_len, pages, int(n_tokens)
         self.struct = KvBatchStruct(n, self.n_tokens, pages.shape[1], q_start.data_ptr(), kv_len.data_ptr(),
                                     pages.data_ptr())

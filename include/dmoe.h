@@ -284,7 +284,8 @@ typedef struct dmoe_kv_cache {
  * (rows outside 0 .. n_tokens, kv_len below its number of rows or above 2^30)
  * is treated as one without rows, and so is one that starts below an earlier
  * entry of q_start.  The three tables are read on the stream: a captured call
- * sees what they hold at each replay. */
+ * sees what they hold at each replay.  n_seqs is at most 2^20, n_tokens and
+ * n_seqs times n_head + 2 n_head_kv at most 2^27 and 2^24. */
 typedef struct dmoe_kv_batch {
     int32_t n_seqs;
     int32_t n_tokens;            /* rows of the token buffers                 */
@@ -306,11 +307,11 @@ typedef struct dmoe_kv_batch {
  * how a denoising step writes its block again and how a cache is cut back.
  * DMOE_KV_E4M3: rows that begin a block set its exponents anew, the least with
  * amax <= 448 * 2^exp; rows that begin inside one keep the tokens before them,
- * whose codes are rounded again where the exponent has to grow.  Two sequences
- * of one call must not write into the same block of the same page.
+ * whose codes are rounded again where the exponent has to grow.  One call must
+ * not write twice into the same block of the same page.
  * ap: n_embd, block_length are not used.  qkv_dev
- * [n_tokens][(n_head + 2 n_head_kv) head_dim] f32 and q_out_dev do not overlap
- * and are 16-byte aligned.  Queued on `stream` without synchronising; uses no
+ * [n_tokens][(n_head + 2 n_head_kv) head_dim] f32 and q_out_dev overlap neither
+ * each other nor the cache and are 16-byte aligned.  Queued on `stream` without synchronising; uses no
  * workspace. */
 int  dmoe_kv_append_device(dmoe_ctx *ctx, const dmoe_kv_cache *kv, const dmoe_kv_batch *batch,
                            const dmoe_attn_hparams *ap, const float *qkv_dev,
@@ -323,7 +324,8 @@ int  dmoe_kv_append_device(dmoe_ctx *ctx, const dmoe_kv_cache *kv, const dmoe_kv
  * scale 1 / sqrt(head_dim), query head h on kv head h / (n_head / n_head_kv);
  * a query that sees nothing gives zeros, and what a query does not see has no
  * part in its result whatever it holds.  q_dev, out_dev
- * [n_tokens][n_head][head_dim] f32, 16-byte aligned, not overlapping; sums and
+ * [n_tokens][n_head][head_dim] f32, 16-byte aligned, out_dev apart from q_dev
+ * and the cache; rows that no sequence has are left as they are; sums and
  * softmax statistics in f32, at f32's accuracy on the cached values.
  * ap: n_head, n_head_kv, head_dim and block_length are used.
  * workspace_dev: dmoe_kv_attn_workspace bytes (16-byte aligned) that no other call in flight
@@ -342,8 +344,8 @@ size_t dmoe_kv_attn_workspace(dmoe_ctx *ctx, const dmoe_kv_cache *kv, const dmoe
  * and projected, their keys and values appended, and they attend to their own
  * sequences' cached tokens; then the output projection, the residual and the
  * post-attention norm.  Positions are the batch's.  h, h_out
- * [n_tokens][n_embd] (h_out may be h); moe_in may be NULL; rows past the last
- * sequence's get no attention and hold nothing of use.  Workspace as for
+ * [n_tokens][n_embd] (h_out may be h); moe_in may be NULL; in h_out and moe_in
+ * rows that no sequence has hold nothing of use.  Workspace as for
  * dmoe_kv_attn_device, dmoe_attn_cached_workspace bytes. */
 int  dmoe_attn_forward_cached_device(dmoe_ctx *ctx, const dmoe_layer *attn, const dmoe_kv_cache *kv,
                                      const dmoe_kv_batch *batch, const float *h_dev,

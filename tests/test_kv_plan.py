@@ -80,7 +80,8 @@ def _call(op, **kw):
 def test_good_arguments_pass(ask):
     calls = [_call(op, **kw) for op in ("append", "attn", "layer", "sizes")
              for kw in ({}, dict(type=0, k_exp=0, v_exp=0), dict(head_dim=64, ap_hd=64), dict(n_head=4), dict(n_tokens=1),
-                        dict(page_tokens=32), dict(block_length=0), dict(block_length=-1), dict(rotary_dim=0),
+                        dict(n_tokens=(1 << 27) // 40, x=20 << 32, y=90 << 32, z=160 << 32), dict(n_seqs=(1 << 24) // 40),
+                        dict(y=(2 << 32) + 10 * 4 * 64 * 128), dict(page_tokens=32), dict(block_length=0), dict(block_length=-1), dict(rotary_dim=0),
                         dict(rotary_dim=128, head_dim=128))]
     calls += [_call("append", use_qk_norm=0, z=0, w=0), _call("layer", z=0), _call("layer", y=GOOD["x"])]
     for c, r in zip(calls, ask(calls)):
@@ -109,6 +110,12 @@ REFUSED = [
     ("append", BAD, dict(z=0)), ("append", BAD, dict(w=0)), ("append", BAD, dict(z=(10 << 32) + 2)),
     ("append", BAD, dict(y=8 << 32)), ("append", BAD, dict(y=(8 << 32) + 33 * 40 * 128 * 4 - 16)),
     ("layer", BAD, dict(z=8 << 32)), ("layer", BAD, dict(z=9 << 32)), ("layer", BAD, dict(z=(10 << 32) + 4)),
+    ("append attn layer sizes", SHAPE, dict(n_tokens=(1 << 27) // 40 + 1)),
+    ("append attn layer sizes", SHAPE, dict(n_seqs=(1 << 24) // 40 + 1)),
+    ("append attn layer sizes", SHAPE, dict(n_tokens=(1 << 31) - 1, n_head=(1 << 31) - 1, ap_kv=(1 << 31) - 1, n_head_kv=(1 << 31) - 1)),
+    ("append attn layer", BAD, dict(y=(1 << 32) + 16)), ("append attn layer", BAD, dict(y=(2 << 32) + 10 * 4 * 64 * 128 - 16)),
+    ("append attn layer", BAD, dict(y=3 << 32)), ("append attn layer", BAD, dict(y=(4 << 32) - 16)),
+    ("append layer", BAD, dict(x=(1 << 32) - 16)), ("layer", BAD, dict(z=2 << 32)),
     ("append layer", SHAPE, dict(rotary_dim=130)), ("append layer", SHAPE, dict(rotary_dim=63)),
     ("append layer", SHAPE, dict(rotary_dim=-2)), ("append layer", BAD, dict(rope_base=0)),
     ("append layer", BAD, dict(rope_base=-1)), ("append layer", BAD, dict(rms_eps=-1)),
@@ -184,3 +191,19 @@ def test_structs_lie_as_in_c(tmp_path):
     got = [int(x) for x in subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True, check=True).stdout.split()]
     want = [x for _, c in pairs for x in [ctypes.sizeof(c)] + [getattr(c, f).offset for f, _ in c._fields_]]
     assert got == want
+
+
+def test_tensors_that_the_mirror_refuses():
+    """Caches and batches of tensors that are not on a GPU, of other types, shapes or strides."""
+    import dmoe
+    import torch
+    k = torch.zeros(3, 2, 64, 64, dtype=torch.float16)
+    v = torch.zeros(3, 2, 2, 64, 32, dtype=torch.float16)
+    i = lambda *shape: torch.zeros(shape, dtype=torch.int32)  # noqa: E731
+    for make in (lambda: dmoe.KvCache(k, v), lambda: dmoe.KvCache(k[0], v), lambda: dmoe.KvCache(k, v[:, :, :1]),
+                 lambda: dmoe.KvCache(k.float(), v), lambda: dmoe.KvCache(k, v.transpose(3, 4)),
+                 lambda: dmoe.KvCache(k[:, :, :40], v), lambda: dmoe.KvBatch(i(3), i(2), i(2, 4), 9),
+                 lambda: dmoe.KvBatch(i(2), i(2), i(2, 4), 9), lambda: dmoe.KvBatch(i(3), i(2), i(3, 4), 9),
+                 lambda: dmoe.KvBatch(i(3), i(2).long(), i(2, 4), 9), lambda: dmoe.KvBatch(i(3), i(2), i(4, 2).T, 9)):
+        with pytest.raises(ValueError):
+            make()
