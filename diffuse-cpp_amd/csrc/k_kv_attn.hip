@@ -368,17 +368,23 @@ struct KvWave {
     // Where a lane's pieces of a tile lie, in bytes from the tile's keys or
     // values.  Row r of key block kb is token 8 (r / 4) + 4 kb + r % 4, so that
     // the scores of a lane are those of tokens 8 g + 4 kb + i.
-    __device__ __forceinline__ uint32_t key_at() const
+    static __device__ __forceinline__ uint32_t key_at()
     {
-        uint32_t at = ((8 * (r16 >> 2) + (r16 & 3)) * HD + 16 * g) * EB;
-        asm volatile("" : "+v"(at));
-        return at;
+        const uint32_t l = lane_again(), r = l & 15;
+        return ((8 * (r >> 2) + (r & 3)) * HD + 16 * (l >> 4)) * EB;
     }
-    __device__ __forceinline__ uint32_t value_at() const
+    static __device__ __forceinline__ uint32_t value_at()
     {
-        uint32_t at = (r16 * 4 + g) * 16;
-        asm volatile("" : "+v"(at));
-        return at;
+        const uint32_t l = lane_again();
+        return ((l & 15) * 4 + (l >> 4)) * 16;
+    }
+    // The lane, formed anew: a few instructions per tile instead of a register
+    // held through the loop, or, worse, a load of a spilled one.
+    static __device__ __forceinline__ uint32_t lane_again()
+    {
+        uint32_t l;
+        asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+        return l;
     }
     static __device__ __forceinline__ uint4 key_piece(Bytes tile, uint32_t at, int i)
     {
@@ -664,13 +670,13 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
     uint4 kr[NK], vr[NK];
     auto load_k = [&](size_t byte) {
         const typename Wave::Bytes tile = Wave::at(a.c.k, byte);
-        const uint32_t at = wave.key_at();
+        const uint32_t at = Wave::key_at();
 #pragma unroll
         for (int i = 0; i < NK; i++) kr[i] = Wave::key_piece(tile, at, i);
     };
     auto load_v = [&](size_t byte) {
         const typename Wave::Bytes tile = Wave::at(a.c.v, byte);
-        const uint32_t at = wave.value_at();
+        const uint32_t at = Wave::value_at();
 #pragma unroll
         for (int i = 0; i < NK; i++) vr[i] = Wave::value_piece(tile, at, i);
     };
@@ -818,12 +824,15 @@ __global__ __launch_bounds__(KW_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
     __shared__ __align__(16) kv_h8 s_kv[2][(2 * NC + NB) * 64];
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int G = a.nh / a.nkv, kvh = blockIdx.x % a.nkv;
+    // The last column tiles see the most: they start first, and of the workgroups
+    // that start at once the second of a CU is the shorter the longer its first.
+    const int places = min((int)gridDim.x, KA_ITEMS), block = blockIdx.x;
+    const int rank = block >= KA_ITEMS / 2 && block < places ? KA_ITEMS / 2 + places - 1 - block : block;
+    const int G = a.nh / a.nkv, kvh = rank % a.nkv;
     int s, tile;
     KvSeq q;
     const int per = 16 * CB * KW_WAVES;
-    // the last column tiles see the most: they start first
-    if (!kv_find(a.b, gridDim.x / a.nkv - 1 - blockIdx.x / a.nkv,
+    if (!kv_find(a.b, (int)gridDim.x / a.nkv - 1 - rank / a.nkv,
                  [&](const KvSeq &r) { return kv_is_wide(a, r, G) ? (r.n * G + per - 1) / per : 0; }, s, q, tile))
         return;
     const int col0 = tile * per + w * 16 * CB;
@@ -836,7 +845,7 @@ __global__ __launch_bounds__(KW_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
     // wavefronts 0 and 1: keys, 2 and 3: values
     auto load = [&](size_t byte) {
         const typename Wave::Bytes tile = Wave::at(w < KW_WAVES / 2 ? a.c.k : a.c.v, byte);
-        const uint32_t at = w < KW_WAVES / 2 ? wave.key_at() : wave.value_at();
+        const uint32_t at = w < KW_WAVES / 2 ? Wave::key_at() : Wave::value_at();
 #pragma unroll
         for (int j = 0; j < NP; j++)
             r[j] = w < KW_WAVES / 2 ? Wave::key_piece(tile, at, w * NP + j) : Wave::value_piece(tile, at, w * NP + j - NK);
@@ -898,6 +907,7 @@ __global__ __launch_bounds__(KW_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
                 }
                 walk.next();
                 load(walk.byte());
+                __builtin_amdgcn_sched_barrier(0);             // not later, for fewer registers
                 wave.template weights<FULL>(st);
                 wave.template add<FULL>(st, [&](auto once, int p, kv_h8(&vf)[NE]) {
                     int at = lane;
