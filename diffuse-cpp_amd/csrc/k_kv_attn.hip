@@ -46,13 +46,14 @@ constexpr int KA_CHUNK = 4;
 constexpr int KA_ITEMS = 512;
 // Columns of all kv heads from which on k_kv_attn_wide runs, a workgroup for 128
 // of them: it reads a token tile once for them, where k_kv_attn does it for 32, but
-// needs a workgroup on most CUs twice.  A prompt of 2000 rows 109 against 128 in
-// F16, 102 against 99 in E4M3, on 4000 cached tokens 312 against 348; of 1024 rows
-// 60 against 55 and 54 against 43.
-constexpr int KA_WIDE = 57344;
+// needs a workgroup on every CU, two for E4M3 whose tiles are half the bytes.
+// Prompts of 1024, 1536 and 2000 rows, wide against not: F16 50 / 56, 69 / 87,
+// 89 / 129, E4M3 47 / 43, 67 / 68, 86 / 99; 1024 rows beside 48 of one on 1000
+// tokens 77 / 68 and 69 / 49, beside 16 blocks of 32 on 2048 104 / 106 and 99 / 80.
+constexpr int KA_WIDE_F16 = 32768, KA_WIDE_E4M3 = 49152;
 // Beside others it takes sequences with fewer columns than that if they have up to
 // KA_LONG token tiles, for it does not cut them: 31 blocks of 32 rows on 1024
-// tokens and one on 32,768 take 131 (F16) and 106 (E4M3), with 16 tiles 390 and 332,
+// tokens and one on 32,768 take 119 (F16) and 97 (E4M3), with 16 tiles 390 and 332,
 // with no limit 1495 and 1433.
 constexpr int KA_LONG = 64;
 
@@ -127,11 +128,16 @@ __device__ __forceinline__ int kv_token_tiles(const KvAttnArgs &a, const KvSeq &
     return q.n ? (kv_cached(q.len, a.c.T, a.b.max_pages) + 31) / 32 : 0;
 }
 
+__host__ __device__ __forceinline__ int kv_wide_from(const KvAttnArgs &a)
+{
+    return a.c.type == DMOE_KV_E4M3 ? KA_WIDE_E4M3 : KA_WIDE_F16;
+}
+
 // Whether k_kv_attn_wide takes a sequence of a call in which it runs.
 __device__ __forceinline__ bool kv_is_wide(const KvAttnArgs &a, const KvSeq &q, int G)
 {
     const int cols = q.n * G;
-    return cols > a.wide && (a.wide == 0 || cols * a.nkv >= KA_WIDE || kv_token_tiles(a, q) <= KA_LONG);
+    return cols > a.wide && (a.wide == 0 || cols * a.nkv >= kv_wide_from(a) || kv_token_tiles(a, q) <= KA_LONG);
 }
 
 __device__ __forceinline__ int kv_col_tiles(const KvAttnArgs &a, const KvSeq &q, int G)
@@ -812,8 +818,11 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
 // left in LDS as operands (lane-contiguous: no bank conflicts); the next tile's
 // loads are in flight during its products.  The queries stay in registers.
 // Bound by the products: 2000 rows on 4001 cached tokens and themselves, 328 GFLOP
-// with both halves, in 276 to 284 us, 1,160 to 1,190 TFLOP/s, which is what a large
-// f16 product of the library reaches here.
+// with both halves, in 270 us, 1,215 TFLOP/s, where a large f16 product of the
+// library reaches 1,160 to 1,310.  A tile takes a wavefront 3,270 cycles, two of
+// them on a SIMD: 1,024 of its MFMAs each, of which 8 cycles apiece are lost to
+// its about 140 other vector instructions (measured apart: 16 MFMAs beside 64 fma
+// of another wavefront take 384 us where either alone takes 265).
 template <int HD, bool F8>
 __global__ __launch_bounds__(KW_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
 {
@@ -1038,12 +1047,12 @@ static KvAttnPlan kv_attn_plan(const KvAttnArgs &a)
     KvAttnPlan p;
     const int64_t cols = (int64_t)a.b.n_tokens * (a.nh / a.nkv);
     const int64_t seqs = std::min(a.b.n_seqs, a.b.n_tokens);       // .. with rows
-    const bool many = cols * a.nkv >= KA_WIDE;
+    const bool many = cols * a.nkv >= kv_wide_from(a);
     p.wide = many ? (seqs == 1 ? 0 : 32 * KW_WAVES) : 0x7fffffff;
     p.wide_items = many ? (cols / (32 * KW_WAVES) + seqs) * a.nkv : 0;
     // a sequence of c columns has at most c / 32 + 1 column tiles, and one that
     // is not k_kv_attn_wide's has not more than these columns
-    const int64_t most = std::max<int64_t>(KA_WIDE / a.nkv, 32 * KW_WAVES);
+    const int64_t most = std::max<int64_t>(kv_wide_from(a) / a.nkv, 32 * KW_WAVES);
     const int64_t tiles = p.wide == 0 ? 0 : std::min(cols / KA_COLS + seqs, many ? seqs * (most / KA_COLS + 1) : cols + seqs);
     p.split = tiles > 0 && (int64_t)a.b.max_pages * (a.c.T / 32) > KA_WHOLE;
     // chunks: less than one more per unit than its share of those wanted
