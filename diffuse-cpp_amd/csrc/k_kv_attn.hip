@@ -49,8 +49,9 @@ constexpr int KA_ITEMS = 512;
 // needs a workgroup on every CU, two for E4M3 whose tiles are half the bytes.
 // Prompts of 1024, 1536 and 2000 rows, wide against not: F16 50 / 56, 69 / 87,
 // 89 / 129, E4M3 47 / 43, 67 / 68, 86 / 99; 1024 rows beside 48 of one on 1000
-// tokens 77 / 68 and 69 / 49, beside 16 blocks of 32 on 2048 104 / 106 and 99 / 80.
-constexpr int KA_WIDE_F16 = 32768, KA_WIDE_E4M3 = 49152;
+// tokens 77 / 68 and 69 / 49, beside 16 blocks of 32 on 2048 104 / 106 and 99 / 80,
+// 1792 beside 8 103 / 133 and 100 / 101.
+constexpr int KA_WIDE_F16 = 32768, KA_WIDE_E4M3 = 57344;
 // Beside others it takes sequences with fewer columns than that if they have up to
 // KA_LONG token tiles, for it does not cut them: 31 blocks of 32 rows on 1024
 // tokens and one on 32,768 take 119 (F16) and 97 (E4M3), with 16 tiles 390 and 332,
