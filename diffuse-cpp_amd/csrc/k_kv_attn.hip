@@ -52,11 +52,14 @@ constexpr int KA_ITEMS = 512;
 // tokens 77 / 68 and 69 / 49, beside 16 blocks of 32 on 2048 104 / 106 and 99 / 80,
 // 1792 beside 8 103 / 133 and 100 / 101.
 constexpr int KA_WIDE_F16 = 32768, KA_WIDE_E4M3 = 57344;
-// Beside others it takes sequences with fewer columns than that if they have up to
-// KA_LONG token tiles, for it does not cut them: 31 blocks of 32 rows on 1024
-// tokens and one on 32,768 take 119 (F16) and 97 (E4M3), with 16 tiles 390 and 332,
-// with no limit 1495 and 1433.
-constexpr int KA_LONG = 64;
+// It does not cut a sequence's tokens, so beside others it takes those with up to
+// KA_LONG token tiles or 1 / KA_SHARE of the tiles of all its workgroups (an item's
+// share is 1 / KA_ITEMS), which no one waits for long.  31 blocks of 32 rows on
+// 1024 tokens and one on 32,768: 115 (F16) and 100 (E4M3), with KA_LONG 16 390 and
+// 332, without a limit 1495 and 1433; four times 512 rows on 4000 tokens 270 and
+// 258, cut 401 and 283; prompts of 2000, 500 on 6000 and 300 on 1000 252 and 209,
+// all of them taken (a 256th) 263 and 262.
+constexpr int KA_LONG = 64, KA_SHARE = 384;
 
 // one 16-byte piece of cache as f16: F16 8 values, E4M3 16
 template <bool F8>
@@ -129,28 +132,37 @@ __device__ __forceinline__ int kv_token_tiles(const KvAttnArgs &a, const KvSeq &
     return q.n ? (kv_cached(q.len, a.c.T, a.b.max_pages) + 31) / 32 : 0;
 }
 
-__host__ __device__ __forceinline__ int kv_wide_from(const KvAttnArgs &a)
+// The most token tiles of a sequence that k_kv_attn_wide takes beside others.
+__device__ __forceinline__ float kv_longest(const KvAttnArgs &a, int G)
 {
-    return a.c.type == DMOE_KV_E4M3 ? KA_WIDE_E4M3 : KA_WIDE_F16;
+    if (a.wide == 0 || a.wide == 0x7fffffff) return 0.0f;
+    float work = 0.0f;
+    for (int base = 0, top = 0; base < a.b.n_seqs; base += 64) {
+        const KvSeq q = kv_seqs(a.b, base, top);
+        const int cols = q.n * G;
+        if (cols > a.wide) work += (float)((cols + 32 * KW_WAVES - 1) / (32 * KW_WAVES)) * (float)kv_token_tiles(a, q);
+    }
+    work = kv_wave_last(kv_wave_scan(work)) * (float)a.nkv;
+    return fmaxf((float)KA_LONG, work * (1.0f / (float)KA_SHARE));
 }
 
 // Whether k_kv_attn_wide takes a sequence of a call in which it runs.
-__device__ __forceinline__ bool kv_is_wide(const KvAttnArgs &a, const KvSeq &q, int G)
+__device__ __forceinline__ bool kv_is_wide(const KvAttnArgs &a, const KvSeq &q, int G, float longest)
 {
-    const int cols = q.n * G;
-    return cols > a.wide && (a.wide == 0 || cols * a.nkv >= kv_wide_from(a) || kv_token_tiles(a, q) <= KA_LONG);
+    return q.n * G > a.wide && (a.wide == 0 || (float)kv_token_tiles(a, q) <= longest);
 }
 
-__device__ __forceinline__ int kv_col_tiles(const KvAttnArgs &a, const KvSeq &q, int G)
+__device__ __forceinline__ int kv_col_tiles(const KvAttnArgs &a, const KvSeq &q, int G, float longest)
 {
     const int cols = q.n * G, per = 16 * kv_blocks_of_tile(cols);
-    return kv_is_wide(a, q, G) ? 0 : (cols + per - 1) / per;
+    return kv_is_wide(a, q, G, longest) ? 0 : (cols + per - 1) / per;
 }
 
 // Item `item` of the call, or false past the last.  One wavefront, 64
 // sequences at a time.
 __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, KvItem &it)
 {
+    const float longest = kv_longest(a, G);
     int top = 0;
     KvSeq q = kv_seqs(a.b, 0, top);
     // f(first sequence) with q a lane's of 64 sequences, until it returns true;
@@ -170,7 +182,7 @@ __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, Kv
         // their pairs of tiles (exact enough: lengths, not indexes)
         float few = 0.0f, many = 0.0f, rest = 0.0f, work = 0.0f;
         each([&](int) {
-            const float tiles = (float)kv_col_tiles(a, q, G);
+            const float tiles = (float)kv_col_tiles(a, q, G, longest);
             const int length = kv_token_tiles(a, q);
             (length > KA_WHOLE ? many : few) += tiles;
             (length > KA_WHOLE ? work : rest) += tiles * (float)length;
@@ -191,7 +203,7 @@ __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, Kv
         float count = 0.0f;
         each([&](int) {
             const int length = kv_token_tiles(a, q);
-            if (length > KA_WHOLE) count += (float)(kv_col_tiles(a, q, G) * (int)((uint32_t)(length + C - 1) / (uint32_t)C));
+            if (length > KA_WHOLE) count += (float)(kv_col_tiles(a, q, G, longest) * (int)((uint32_t)(length + C - 1) / (uint32_t)C));
             return false;
         });
         count = kv_wave_last(kv_wave_scan(count));
@@ -200,7 +212,7 @@ __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, Kv
     }
     int parts = 0, units = 0;
     if (each([&](int base) {
-            const int tiles = kv_col_tiles(a, q, G), length = kv_token_tiles(a, q);
+            const int tiles = kv_col_tiles(a, q, G, longest), length = kv_token_tiles(a, q);
             // (one without tokens still has its rows to zero)
             const int ks = length > KA_WHOLE ? (int)((uint32_t)(length + C - 1) / (uint32_t)C) : 1;
             const int count = tiles * ks * a.nkv, part = ks > 1 ? tiles * ks : 0, unit = ks > 1 ? tiles : 0;
@@ -842,8 +854,9 @@ __global__ __launch_bounds__(KW_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
     int s, tile;
     KvSeq q;
     const int per = 16 * CB * KW_WAVES;
+    const float longest = kv_longest(a, G);
     if (!kv_find(a.b, (int)gridDim.x / a.nkv - 1 - rank / a.nkv,
-                 [&](const KvSeq &r) { return kv_is_wide(a, r, G) ? (r.n * G + per - 1) / per : 0; }, s, q, tile))
+                 [&](const KvSeq &r) { return kv_is_wide(a, r, G, longest) ? (r.n * G + per - 1) / per : 0; }, s, q, tile))
         return;
     const int col0 = tile * per + w * 16 * CB;
     Wave wave;
@@ -1048,12 +1061,12 @@ static KvAttnPlan kv_attn_plan(const KvAttnArgs &a)
     KvAttnPlan p;
     const int64_t cols = (int64_t)a.b.n_tokens * (a.nh / a.nkv);
     const int64_t seqs = std::min(a.b.n_seqs, a.b.n_tokens);       // .. with rows
-    const bool many = cols * a.nkv >= kv_wide_from(a);
+    const bool many = cols * a.nkv >= (a.c.type == DMOE_KV_E4M3 ? KA_WIDE_E4M3 : KA_WIDE_F16);
     p.wide = many ? (seqs == 1 ? 0 : 32 * KW_WAVES) : 0x7fffffff;
     p.wide_items = many ? (cols / (32 * KW_WAVES) + seqs) * a.nkv : 0;
     // a sequence of c columns has at most c / 32 + 1 column tiles, and one that
-    // is not k_kv_attn_wide's has not more than these columns
-    const int64_t most = std::max<int64_t>(kv_wide_from(a) / a.nkv, 32 * KW_WAVES);
+    // is not k_kv_attn_wide's has less than the columns of KA_SHARE workgroups
+    const int64_t most = (KA_SHARE / a.nkv + 1) * (int64_t)(32 * KW_WAVES);
     const int64_t tiles = p.wide == 0 ? 0 : std::min(cols / KA_COLS + seqs, many ? seqs * (most / KA_COLS + 1) : cols + seqs);
     p.split = tiles > 0 && (int64_t)a.b.max_pages * (a.c.T / 32) > KA_WHOLE;
     // chunks: less than one more per unit than its share of those wanted

@@ -68,6 +68,7 @@ def _check(batch, cache, q, block, got):
 GROUPS = {
     "one": [(0, 1800)], "after": [(90, 1795)], "long": [(2500, 1830)],
     "beside": [(5, 3), (0, 0), (2100, 513), (700, 1), (31, 16), (0, 17), (63, 70), (1, 1150), (900, 33)],
+    "full": [(10, 2300)],                            # more workgroups than start at once
     "padded": [(3000, 40)],                          # fewer rows than the buffers hold
     "many": [(i * 397 % 1700, i % 6) for i in range(150)],
 }
