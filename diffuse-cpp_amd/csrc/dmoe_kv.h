@@ -98,6 +98,35 @@ __device__ __forceinline__ bool kv_find(const KvBatch &b, int item, Count &&coun
     return false;
 }
 
+// Block `blk` of sequence `seq` at place `item` of kv_place's list, found by one
+// wavefront, 64 sequences at a time or every 64th part of more; false where a
+// place is empty.  (In a table that decreases it may be any sequence's, or none's.)
+__device__ __forceinline__ bool kv_find_block(const KvBatch &b, int item, int &seq, KvSeq &info, int &blk)
+{
+    const int lane = threadIdx.x & 63;
+    const bool by_row = kv_by_row(b.n_seqs, b.n_tokens);
+    int first = 0, n = b.n_seqs;
+    while (n > 64) {
+        const int part = (n + 63) / 64, i = lane * part;
+        const uint64_t before = __ballot(i < n && kv_place(b.q_start[first + min(i, n - 1)], first + i, by_row) <= item);
+        if (!before) return false;
+        const int k = 63 - __builtin_clzll(before);
+        first += k * part;
+        n = min(part, n - k * part);
+    }
+    KvSeq q{0, 0, 0};
+    if (lane < n) q = kv_seq(b, first + lane);
+    const uint64_t before = __ballot(lane < n && kv_place(q.q0, first + lane, by_row) <= item);
+    if (!before) return false;
+    const int l = 63 - __builtin_clzll(before);
+    seq = first + l;
+    info.q0 = __builtin_amdgcn_readlane(q.q0, l);
+    info.n = __builtin_amdgcn_readlane(q.n, l);
+    info.len = __builtin_amdgcn_readlane(q.len, l);
+    blk = item - kv_place(info.q0, seq, by_row);
+    return blk >= 0 && blk < kv_blocks(info);
+}
+
 // The page that holds token `pos` of sequence s, or -1.
 __device__ __forceinline__ int kv_page(const KvBatch &b, const KvCacheView &c, int s, int pos)
 {

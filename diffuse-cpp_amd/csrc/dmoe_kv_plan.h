@@ -44,12 +44,24 @@ KV_HD int kv_blocks(const KvSeq &q)
     return q.n ? (q.len - 1) / 32 - (q.len - q.n) / 32 + 1 : 0;
 }
 
-// At least the sum of kv_blocks over the sequences of a batch whose rows do not
-// overlap: a sequence of n rows touches at most n, and at most n / 32 + 2.
+// Where a sequence's blocks begin in a list that has room for those of every one,
+// found from its first row alone: a sequence of n rows touches at most n blocks,
+// and at most n / 32 + 2.  `by_row`: a place for each row, else one for each 32 and
+// two for each sequence, whichever is less in all.
+KV_HD bool kv_by_row(int n_seqs, int n_tokens)
+{
+    return n_tokens <= n_tokens / 32 + 2 * (int64_t)n_seqs;
+}
+
+KV_HD int kv_place(int start, int s, bool by_row)
+{
+    return by_row ? start : start / 32 + 2 * s;
+}
+
+// Places of that list: no less than the blocks of a batch.
 KV_HD int64_t kv_blocks_most(int n_seqs, int n_tokens)
 {
-    const int64_t b = n_tokens / 32 + 2 * (int64_t)n_seqs;
-    return b < n_tokens ? b : n_tokens;
+    return kv_by_row(n_seqs, n_tokens) ? n_tokens : n_tokens / 32 + 2 * (int64_t)n_seqs;
 }
 
 // The entry of a sequence's row of the page table for token `pos`, or -1 past

@@ -154,7 +154,13 @@ __global__ __launch_bounds__(KA_WAVES * 64) void k_kv_append(KvAppendArgs a)
     }
     int s, blk;
     KvSeq q;
-    if (!kv_find(a.b, (int)item, [](const KvSeq &r) { return kv_blocks(r); }, s, q, blk)) return;
+    // Up to 64 sequences: their blocks counted, without gaps between them (16 blocks
+    // of 32 rows 7.4 us on end, from their places 9.4).  More: from their places, as
+    // counting takes every workgroup a pass over all of them (4096 rows of as many
+    // sequences 837 us, so 196).
+    if (a.b.n_seqs <= 64 ? !kv_find(a.b, (int)item, [](const KvSeq &r) { return kv_blocks(r); }, s, q, blk)
+                         : !kv_find_block(a.b, (int)item, s, q, blk))
+        return;
     const int pos_q = q.len - q.n;                                   // the first row's position
     const int pos = max(pos_q, (pos_q / 32 + blk) * 32);             // this block's first row
     const int off = pos % 32;

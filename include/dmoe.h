@@ -282,8 +282,9 @@ typedef struct dmoe_kv_cache {
  * (-1, say) and a token past the table hold nothing: an append skips them, the
  * attention does not see them.  A sequence whose numbers contradict each other
  * (rows outside 0 .. n_tokens, kv_len below its number of rows or above 2^30)
- * is treated as one without rows, and so is one that starts below an earlier
- * entry of q_start.  The three tables are read on the stream: a captured call
+ * is treated as one without rows; where q_start decreases, which rows the
+ * sequences from there on have is not defined, but nothing outside the buffers
+ * is touched.  The three tables are read on the stream: a captured call
  * sees what they hold at each replay.  n_seqs is at most 2^20, n_tokens and
  * n_seqs times n_head + 2 n_head_kv at most 2^27 and 2^24. */
 typedef struct dmoe_kv_batch {

@@ -205,9 +205,10 @@ def test_pages_looked_up_several_times(ctx, kvtype):
 
 @pytest.mark.parametrize("n", [2, 1800])
 def test_rows_of_an_earlier_sequence(ctx, n):
-    """Tables that decrease: sequences that start below an earlier entry of
-    q_start have no rows, in the append and in the attention; the others are as
-    without them."""
+    """Tables that decrease, with more work than there are rows: the attention
+    takes the rows of a sequence that starts below an earlier entry of q_start
+    for the earlier one's, and an append stays within the cache (which rows it
+    takes is not defined; here all that it can take hold the same)."""
     import dmoe
     nh, nkv, hd, T = 32, 4, 64, 64
     print(f"case: tables that decrease, {n} rows", flush=True)
@@ -227,11 +228,16 @@ def test_rows_of_an_earlier_sequence(ctx, n):
         kv = cache.device(dmoe)
         q, out = (torch.full((batch.n_tokens, nh, hd), 7.0, device="cuda:0") for _ in range(2))
         ctx.kv_append_device(kv, b, ap, qkv, q)
-        ctx.kv_attn_device(kv, b, ap, q, out)
+        if not more:
+            whole, queries = kv, q
+        ctx.kv_attn_device(whole, b, ap, queries, out)
         torch.cuda.synchronize()
         results.append((R.Cache.of(kv), q.cpu().numpy(), out.cpu().numpy()))
     (c0, q0, o0), (c1, q1, o1) = results
-    assert c0.same(c1) and np.array_equal(q0, q1)
+    # what the second append took is as in the first, the rest as it was
+    for x, y, z in ((c0.k, c1.k, cache.k), (c0.v, c1.v, cache.v)):
+        assert bool(((x == y) | (y == z)).all())
+    assert ((q0 == q1) | (q1 == 7.0)).all()
     ref, top_v, top_s = attend(batch, c0, q0, 1)
     tol = R.attend_tolerance(top_v, top_s, hd, 900 + n)
     assert max(np.abs(o0 - ref).max(), np.abs(o1 - ref).max()) <= tol

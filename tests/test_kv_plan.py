@@ -27,6 +27,8 @@ int main() {
       KvSeq q = kv_seq_of(v[0], v[1], v[2], v[3]);
       printf("%%d %%d %%d %%d\n", q.q0, q.n, q.len, kv_blocks(q));
     } else if (!strcmp(op, "most")) printf("%%lld\n", (long long)kv_blocks_most(v[0], v[1]));
+    else if (!strcmp(op, "byrow")) printf("%%d\n", (int)kv_by_row(v[0], v[1]));
+    else if (!strcmp(op, "place")) printf("%%d\n", kv_place(v[0], v[1], v[2]));
     else if (!strcmp(op, "entry")) printf("%%d\n", kv_entry_of(v[0], v[1], v[2]));
     else if (!strcmp(op, "page")) printf("%%d\n", kv_page_of(v[0], v[1]));
     else if (!strcmp(op, "sees")) printf("%%d\n", kv_visible(v[0], kv_cached(v[1], v[2], v[3]), v[4]));
@@ -207,3 +209,22 @@ def test_tensors_that_the_mirror_refuses():
                  lambda: dmoe.KvBatch(i(3), i(2).long(), i(2, 4), 9), lambda: dmoe.KvBatch(i(3), i(2), i(4, 2).T, 9)):
         with pytest.raises(ValueError):
             make()
+
+
+def test_every_block_has_a_place_of_its_own(ask):
+    """kv_place's list: the blocks of ragged batches, sequences without rows among
+    them, lie in disjoint places within the launch's bound, in order."""
+    rng = random.Random(8)
+    for _ in range(100):
+        seqs = [(rng.choice((0, 1, 31, rng.randrange(5000))), rng.choice((0, 0, 1, 1, 2, 32, 33, rng.randrange(300))))
+                for _ in range(rng.randrange(1, 90))]
+        n = sum(b for _, b in seqs)
+        if n == 0:
+            continue
+        starts = [sum(b for _, b in seqs[:i]) for i in range(len(seqs) + 1)]
+        by_row = int(ask([("byrow", [len(seqs), n])])[0])
+        places = [int(x) for x in ask([("place", [starts[i], i, by_row]) for i in range(len(seqs) + 1)])]
+        most = int(ask([("most", [len(seqs), n])])[0])
+        for i, (o, b) in enumerate(seqs):
+            blocks = (o + b - 1) // 32 - o // 32 + 1 if b else 0
+            assert places[i] + blocks <= places[i + 1] <= most
