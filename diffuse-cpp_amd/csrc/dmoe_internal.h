@@ -268,6 +268,7 @@ struct KvAttnArgs {
     float *out;
     void *ws;
     int32_t units, split, wide;          // set by the launch
+    struct KvGroup *groups;
 };
 hipError_t launch_kv_attn(const KvAttnArgs &a, hipStream_t s);
 // bytes of a.ws that the launch needs; the tables are not read

@@ -132,18 +132,17 @@ __device__ __forceinline__ int kv_token_tiles(const KvAttnArgs &a, const KvSeq &
     return q.n ? (kv_cached(q.len, a.c.T, a.b.max_pages) + 31) / 32 : 0;
 }
 
-// The most token tiles of a sequence that k_kv_attn_wide takes beside others.
-__device__ __forceinline__ float kv_longest(const KvAttnArgs &a, int G)
+// The most token tiles of a sequence that k_kv_attn_wide takes beside others, from
+// the sum of what it could take.
+__device__ __forceinline__ float kv_wide_work(const KvAttnArgs &a, const KvSeq &q, int G)
 {
-    if (a.wide == 0 || a.wide == 0x7fffffff) return 0.0f;
-    float work = 0.0f;
-    for (int base = 0, top = 0; base < a.b.n_seqs; base += 64) {
-        const KvSeq q = kv_seqs(a.b, base, top);
-        const int cols = q.n * G;
-        if (cols > a.wide) work += (float)((cols + 32 * KW_WAVES - 1) / (32 * KW_WAVES)) * (float)kv_token_tiles(a, q);
-    }
-    work = kv_wave_last(kv_wave_scan(work)) * (float)a.nkv;
-    return fmaxf((float)KA_LONG, work * (1.0f / (float)KA_SHARE));
+    const int cols = q.n * G;
+    return cols > a.wide ? (float)((cols + 32 * KW_WAVES - 1) / (32 * KW_WAVES)) * (float)kv_token_tiles(a, q) : 0.0f;
+}
+
+__device__ __forceinline__ float kv_longest(const KvAttnArgs &a, float work)
+{
+    return fmaxf((float)KA_LONG, work * (float)a.nkv * (1.0f / (float)KA_SHARE));
 }
 
 // Whether k_kv_attn_wide takes a sequence of a call in which it runs.
@@ -158,88 +157,127 @@ __device__ __forceinline__ int kv_col_tiles(const KvAttnArgs &a, const KvSeq &q,
     return kv_is_wide(a, q, G, longest) ? 0 : (cols + per - 1) / per;
 }
 
-// Item `item` of the call, or false past the last.  One wavefront, 64
-// sequences at a time.
+// Column tiles of the sequences that are not cut and of the others, and their pairs
+// of tiles (exact enough: lengths, not indexes).
+struct KvWork {
+    float few, many, rest, work;
+};
+__device__ __forceinline__ void kv_add_work(const KvAttnArgs &a, const KvSeq &q, int G, float longest, KvWork &sum)
+{
+    const float tiles = (float)kv_col_tiles(a, q, G, longest);
+    const int length = kv_token_tiles(a, q);
+    (length > KA_WHOLE ? sum.many : sum.few) += tiles;
+    (length > KA_WHOLE ? sum.work : sum.rest) += tiles * (float)length;
+}
+
+// Chunks of a sequence.
+__device__ __forceinline__ int kv_cuts(int length, int C)
+{
+    return length > KA_WHOLE ? (int)((uint32_t)(length + C - 1) / (uint32_t)C) : 1;
+}
+
+// The chunk length.  What all can start at once is shared out; a column tile's last
+// chunk is half empty on average, and where that is not enough the count of chunks
+// says by how much.  If that would make a chunk twice as long as an item's share of
+// all the work, the items start one after the other anyhow, and the share it is.
+__device__ __forceinline__ float kv_chunk(const KvAttnArgs &a, const KvWork &sum)
+{
+    const float all = (float)KA_ITEMS / (float)a.nkv;
+    return sum.work / fmaxf(all - sum.few - 0.5f * sum.many, 0.25f * all) + 1.0f;
+}
+__device__ __forceinline__ float kv_chunks(const KvAttnArgs &a, const KvSeq &q, int G, float longest, float c)
+{
+    const int length = kv_token_tiles(a, q), C = max(KA_CHUNK, (int)c);
+    return length > KA_WHOLE ? (float)(kv_col_tiles(a, q, G, longest) * kv_cuts(length, C)) : 0.0f;
+}
+__device__ __forceinline__ int kv_chunk(const KvAttnArgs &a, const KvWork &sum, float c, float count)
+{
+    const float all = (float)KA_ITEMS / (float)a.nkv, share = (sum.work + sum.rest) / all + 1.0f;
+    if (count > all - sum.few) c = fmaxf(fmaxf((float)KA_CHUNK, floorf(c)), c * count / fmaxf(all - sum.few, 0.25f * all) + 1.0f);
+    return max(KA_CHUNK, (int)(c > 2.0f * share ? share : c));
+}
+
+// What lies at the start of the workspace, and, of more than 64 sequences, what
+// comes before each 64 of them (k_kv_list).  Else each workgroup would pass over all
+// of them: 1024 rows of as many sequences of 1000 tokens take 161 us with the list,
+// 357 without, 4096 of 200 353 and 3041, 256 of 200 28 and 24.
+struct KvHeader {
+    int32_t units;                       // of the join: written by k_kv_attn
+    int32_t C;
+    float longest;
+    int32_t pad[5];
+};
+struct KvGroup {
+    int32_t items, parts, units, wide, top;              // wide: items of k_kv_attn_wide
+    int32_t pad[3];
+};
+
+// The last group with key(group) <= item, its first sequence in `base`.
+template <class Key>
+__device__ __forceinline__ KvGroup kv_group(const KvAttnArgs &a, int item, Key &&key, int &base)
+{
+    const int lane = threadIdx.x & 63;
+    int first = 0, n = (a.b.n_seqs + 63) / 64;
+    while (n > 1) {
+        const int part = (n + 63) / 64, i = lane * part;
+        const uint64_t before = __ballot(i < n && key(a.groups[first + min(i, n - 1)]) <= item);
+        const int k = 63 - __builtin_clzll(before | 1);
+        first += k * part;
+        n = min(part, n - k * part);
+    }
+    base = 64 * first;
+    return a.groups[first];
+}
+
+// Item `item` of the call, or false past the last.  One wavefront.
 __device__ __forceinline__ bool kv_item(const KvAttnArgs &a, int G, int item, KvItem &it)
 {
-    const float longest = kv_longest(a, G);
-    int top = 0;
-    KvSeq q = kv_seqs(a.b, 0, top);
-    // f(first sequence) with q a lane's of 64 sequences, until it returns true;
-    // of up to 64 they are read once
-    auto each = [&](auto &&f) {
-        if (a.b.n_seqs <= 64) return f(0);
-        top = 0;
-        for (int base = 0; base < a.b.n_seqs; base += 64) {
-            q = kv_seqs(a.b, base, top);
-            if (f(base)) return true;
-        }
-        return false;
-    };
-    int C = 0x7fffffff;
-    if (a.split) {
-        // column tiles of the sequences that are not cut and of the others, and
-        // their pairs of tiles (exact enough: lengths, not indexes)
-        float few = 0.0f, many = 0.0f, rest = 0.0f, work = 0.0f;
-        each([&](int) {
-            const float tiles = (float)kv_col_tiles(a, q, G, longest);
-            const int length = kv_token_tiles(a, q);
-            (length > KA_WHOLE ? many : few) += tiles;
-            (length > KA_WHOLE ? work : rest) += tiles * (float)length;
-            return false;
-        });
-        few = kv_wave_last(kv_wave_scan(few));
-        many = kv_wave_last(kv_wave_scan(many));
-        rest = kv_wave_last(kv_wave_scan(rest));
-        work = kv_wave_last(kv_wave_scan(work));
-        // What all can start at once is shared out; a column tile's last chunk
-        // is half empty on average, and where that is not enough the count
-        // says by how much.  If that would make a chunk twice as long as an
-        // item's share of all the work, the items start one after the other
-        // anyhow, and the share it is.
-        const float all = (float)KA_ITEMS / (float)a.nkv, share = (work + rest) / all + 1.0f;
-        float c = work / fmaxf(all - few - 0.5f * many, 0.25f * all) + 1.0f;
-        C = max(KA_CHUNK, (int)c);
-        float count = 0.0f;
-        each([&](int) {
-            const int length = kv_token_tiles(a, q);
-            if (length > KA_WHOLE) count += (float)(kv_col_tiles(a, q, G, longest) * (int)((uint32_t)(length + C - 1) / (uint32_t)C));
-            return false;
-        });
-        count = kv_wave_last(kv_wave_scan(count));
-        if (count > all - few) c = fmaxf((float)C, c * count / fmaxf(all - few, 0.25f * all) + 1.0f);
-        C = max(KA_CHUNK, (int)(c > 2.0f * share ? share : c));
+    int base = 0, top = 0, parts = 0, units = 0;
+    float longest = 0.0f;
+    if (a.b.n_seqs > 64) {
+        const KvGroup g = kv_group(a, item, [](const KvGroup &r) { return r.items; }, base);
+        top = g.top;
+        item -= g.items;
+        parts = g.parts;
+        units = g.units;
+        longest = ((const KvHeader *)a.ws)->longest;
     }
-    int parts = 0, units = 0;
-    if (each([&](int base) {
-            const int tiles = kv_col_tiles(a, q, G, longest), length = kv_token_tiles(a, q);
-            // (one without tokens still has its rows to zero)
-            const int ks = length > KA_WHOLE ? (int)((uint32_t)(length + C - 1) / (uint32_t)C) : 1;
-            const int count = tiles * ks * a.nkv, part = ks > 1 ? tiles * ks : 0, unit = ks > 1 ? tiles : 0;
-            const int end = kv_wave_scan(count), parts_end = kv_wave_scan(part), units_end = kv_wave_scan(unit);
-            const uint64_t past = __ballot(end > item);
-            if (!past) {
-                item -= kv_wave_last(end);
-                parts += kv_wave_last(parts_end);
-                units += kv_wave_last(units_end);
-                return false;
-            }
-            const int l = __builtin_ctzll(past);
-            auto at = [&](int v) { return (uint32_t)__builtin_amdgcn_readlane(v, l); };
-            const uint32_t n = at(ks), i = (uint32_t)item - (at(end) - at(count));
-            it.s = base + l;
-            it.q = KvSeq{(int)at(q.q0), (int)at(q.n), (int)at(q.len)};
-            it.cb = kv_blocks_of_tile(it.q.n * G);
-            it.ks = (int)n;
-            it.chunk = (int)((at(length) + n - 1) / n);
-            it.kvh = (int)(i % (uint32_t)a.nkv);
-            it.split = (int)(i / (uint32_t)a.nkv % n);
-            it.tile = (int)(i / (uint32_t)a.nkv / n);
-            it.part = (parts + (int)(at(parts_end) - at(part))) * a.nkv + (int)i;
-            it.unit = (units + (int)(at(units_end) - at(unit)) + it.tile) * a.nkv + it.kvh;
-            return true;
-        }))
+    const KvSeq q = kv_seqs(a.b, base, top);
+    if (a.b.n_seqs <= 64 && a.wide > 0 && a.wide < 0x7fffffff) longest = kv_longest(a, kv_wave_last(kv_wave_scan(kv_wide_work(a, q, G))));
+    int C = 0x7fffffff;
+    if (a.b.n_seqs > 64) {
+        C = ((const KvHeader *)a.ws)->C;
+    } else if (a.split) {
+        KvWork sum{};
+        kv_add_work(a, q, G, longest, sum);
+        sum.few = kv_wave_last(kv_wave_scan(sum.few));
+        sum.many = kv_wave_last(kv_wave_scan(sum.many));
+        sum.rest = kv_wave_last(kv_wave_scan(sum.rest));
+        sum.work = kv_wave_last(kv_wave_scan(sum.work));
+        const float c = kv_chunk(a, sum);
+        C = kv_chunk(a, sum, c, kv_wave_last(kv_wave_scan(kv_chunks(a, q, G, longest, c))));
+    }
+    const int tiles = kv_col_tiles(a, q, G, longest), length = kv_token_tiles(a, q), ks = kv_cuts(length, C);
+    const int count = tiles * ks * a.nkv, part = ks > 1 ? tiles * ks : 0, unit = ks > 1 ? tiles : 0;
+    const int end = kv_wave_scan(count), parts_end = kv_wave_scan(part), units_end = kv_wave_scan(unit);
+    const uint64_t past = __ballot(end > item);
+    if (past) {
+        const int l = __builtin_ctzll(past);
+        auto at = [&](int v) { return (uint32_t)__builtin_amdgcn_readlane(v, l); };
+        const uint32_t n = at(ks), i = (uint32_t)item - (at(end) - at(count));
+        it.s = base + l;
+        it.q = KvSeq{(int)at(q.q0), (int)at(q.n), (int)at(q.len)};
+        it.cb = kv_blocks_of_tile(it.q.n * G);
+        it.ks = (int)n;
+        it.chunk = (int)((at(length) + n - 1) / n);
+        it.kvh = (int)(i % (uint32_t)a.nkv);
+        it.split = (int)(i / (uint32_t)a.nkv % n);
+        it.tile = (int)(i / (uint32_t)a.nkv / n);
+        it.part = (parts + (int)(at(parts_end) - at(part))) * a.nkv + (int)i;
+        it.unit = (units + (int)(at(units_end) - at(unit)) + it.tile) * a.nkv + it.kvh;
         return true;
+    }
+    units += kv_wave_last(units_end);
     it.unit = units * a.nkv;             // how many there are
     return false;
 }
@@ -825,6 +863,86 @@ __device__ __forceinline__ void kv_attend(const KvAttnArgs &a, const KvItem &it,
     }
 }
 
+// The list of more than 64 sequences, in one workgroup, 1024 at a time.
+__global__ __launch_bounds__(1024) void k_kv_list(KvAttnArgs a)
+{
+    __shared__ float s_f[16];
+    __shared__ int s_i[16];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, G = a.nh / a.nkv;
+    // the sum over the workgroup
+    auto total = [&](float v) {
+        v = kv_wave_scan(v);
+        __syncthreads();
+        if (lane == 63) s_f[w] = v;
+        __syncthreads();
+        v = 0.0f;
+        for (int i = 0; i < 16; i++) v += s_f[i];
+        return v;
+    };
+    // op over the wavefronts before this one and `v` (the last one's with it)
+    auto before = [&](int mine, int &v, auto &&op) {
+        __syncthreads();
+        if (lane == 0) s_i[w] = mine;
+        __syncthreads();
+        int r = v;
+        for (int i = 0; i < 16; i++) {
+            if (i < w) r = op(r, s_i[i]);
+            v = op(v, s_i[i]);
+        }
+        return r;
+    };
+    auto most = [](int x, int y) { return max(x, y); };
+    auto sum = [](int x, int y) { return x + y; };
+    // f(first sequence of the wavefront's 64, what came before them), q a lane's
+    KvSeq q;
+    auto each = [&](auto &&f) {
+        int top = 0;
+        for (int base = 0; base < a.b.n_seqs; base += 1024) {
+            int own = 0;
+            (void)kv_seqs(a.b, base + 64 * w, own);
+            int from = before(own, top, most);
+            const int met = from;
+            q = kv_seqs(a.b, base + 64 * w, from);
+            f(base + 64 * w, met);
+        }
+    };
+    float longest = 0.0f;
+    if (a.wide > 0 && a.wide < 0x7fffffff) {
+        float work = 0.0f;
+        each([&](int, int) { work += kv_wide_work(a, q, G); });
+        longest = kv_longest(a, total(work));
+    }
+    int C = 0x7fffffff;
+    if (a.split) {
+        KvWork all{};
+        each([&](int, int) { kv_add_work(a, q, G, longest, all); });
+        all.few = total(all.few);
+        all.many = total(all.many);
+        all.rest = total(all.rest);
+        all.work = total(all.work);
+        const float c = kv_chunk(a, all);
+        float count = 0.0f;
+        each([&](int, int) { count += kv_chunks(a, q, G, longest, c); });
+        C = kv_chunk(a, all, c, total(count));
+    }
+    int items = 0, parts = 0, units = 0, wide = 0;
+    const int per = 32 * KW_WAVES;
+    each([&](int base, int met) {
+        const int tiles = kv_col_tiles(a, q, G, longest), ks = kv_cuts(kv_token_tiles(a, q), C);
+        KvGroup g{};
+        g.top = met;
+        g.items = before(kv_wave_last(kv_wave_scan(tiles * ks * a.nkv)), items, sum);
+        g.parts = before(kv_wave_last(kv_wave_scan(ks > 1 ? tiles * ks : 0)), parts, sum);
+        g.units = before(kv_wave_last(kv_wave_scan(ks > 1 ? tiles : 0)), units, sum);
+        g.wide = before(kv_wave_last(kv_wave_scan(kv_is_wide(a, q, G, longest) ? (q.n * G + per - 1) / per : 0)), wide, sum);
+        if (lane == 0 && base < a.b.n_seqs) a.groups[base / 64] = g;
+    });
+    if (threadIdx.x == 0) {
+        ((KvHeader *)a.ws)->C = C;
+        ((KvHeader *)a.ws)->longest = longest;
+    }
+}
+
 // Many columns of one sequence (prompts): a workgroup takes 32 KW_WAVES of
 // them, each wavefront 32, over all the tokens they see.  A token tile is
 // loaded once for all four wavefronts, a quarter by each, widened to f16 and
@@ -854,10 +972,26 @@ __global__ __launch_bounds__(KW_WAVES * 64, 2) void k_kv_attn_wide(KvAttnArgs a)
     int s, tile;
     KvSeq q;
     const int per = 16 * CB * KW_WAVES;
-    const float longest = kv_longest(a, G);
-    if (!kv_find(a.b, (int)gridDim.x / a.nkv - 1 - rank / a.nkv,
-                 [&](const KvSeq &r) { return kv_is_wide(a, r, G, longest) ? (r.n * G + per - 1) / per : 0; }, s, q, tile))
-        return;
+    int item = (int)gridDim.x / a.nkv - 1 - rank / a.nkv;
+    {
+        int base = 0, top = 0;
+        float longest = 0.0f;
+        if (a.b.n_seqs > 64) {
+            const KvGroup g = kv_group(a, item, [](const KvGroup &r) { return r.wide; }, base);
+            top = g.top;
+            item -= g.wide;
+            longest = ((const KvHeader *)a.ws)->longest;
+        }
+        const KvSeq r = kv_seqs(a.b, base, top);
+        if (a.b.n_seqs <= 64 && a.wide > 0) longest = kv_longest(a, kv_wave_last(kv_wave_scan(kv_wide_work(a, r, G))));
+        const int count = kv_is_wide(a, r, G, longest) ? (r.n * G + per - 1) / per : 0, end = kv_wave_scan(count);
+        const uint64_t past = __ballot(end > item);
+        if (!past) return;
+        const int l = __builtin_ctzll(past);
+        s = base + l;
+        q = KvSeq{__builtin_amdgcn_readlane(r.q0, l), __builtin_amdgcn_readlane(r.n, l), __builtin_amdgcn_readlane(r.len, l)};
+        tile = item - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(count, l));
+    }
     const int col0 = tile * per + w * 16 * CB;
     Wave wave;
     wave.start(a, q, G, col0);
@@ -983,7 +1117,7 @@ __global__ __launch_bounds__(KA_WAVES * 64, 2) void k_kv_attn(KvAttnArgs a)
     KvItem it;
     if (!kv_item(a, G, blockIdx.x, it)) {
         // (the launch's bound on the items is never reached)
-        if (a.split && threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) *(int32_t *)a.ws = it.unit;
+        if (a.split && threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) ((KvHeader *)a.ws)->units = it.unit;
         return;
     }
     if (it.ks > 1 && it.split == 0 && threadIdx.x == 0)
@@ -1003,7 +1137,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_join(KvAttnArgs a)
     constexpr int ND = DIMS / 4, PARTS = THREADS / (COLS * ND);
     __shared__ __align__(16) float4 s_o[PARTS][COLS][ND];
     __shared__ float s_m[PARTS][COLS], s_l[PARTS][COLS];
-    const int units = *(const int32_t *)a.ws;
+    const int units = ((const KvHeader *)a.ws)->units;
     const KvDesc d = ((const KvDesc *)a.ws)[1 + blockIdx.x];
     const int c0 = (int)blockIdx.y / (HD / DIMS) * COLS, d0 = (int)blockIdx.y % (HD / DIMS) * DIMS;
     if ((int)blockIdx.x >= units || c0 >= d.cols) return;
@@ -1054,6 +1188,7 @@ struct KvAttnPlan {
     int64_t units, parts;                // what the workspace holds
     int32_t wide;                        // columns above which a sequence can be k_kv_attn_wide's
     bool split;
+    size_t groups, bytes;                // where the workspace holds the groups, and its size
 };
 
 static KvAttnPlan kv_attn_plan(const KvAttnArgs &a)
@@ -1072,14 +1207,15 @@ static KvAttnPlan kv_attn_plan(const KvAttnArgs &a)
     // chunks: less than one more per unit than its share of those wanted
     p.items = tiles * a.nkv + (p.split ? KA_ITEMS + 1 : 0);
     p.units = std::min<int64_t>(tiles * a.nkv, KA_ITEMS);
-    p.parts = std::min<int64_t>(p.items, 2 * KA_ITEMS);
+    p.parts = p.split ? std::min<int64_t>(p.items, 2 * KA_ITEMS) : 0;
+    p.groups = (size_t)(1 + p.units) * sizeof(KvDesc) + (size_t)p.parts * KA_COLS * (a.hd + 2) * 4;
+    p.bytes = p.groups + (a.b.n_seqs > 64 ? (size_t)(a.b.n_seqs + 63) / 64 * sizeof(KvGroup) : 0);
     return p;
 }
 
 size_t kv_attn_ws_bytes(const KvAttnArgs &a)
 {
-    const KvAttnPlan p = kv_attn_plan(a);
-    return p.split ? (size_t)(1 + p.units) * sizeof(KvDesc) + (size_t)p.parts * KA_COLS * (a.hd + 2) * 4 : 256;
+    return kv_attn_plan(a).bytes;
 }
 
 hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
@@ -1090,6 +1226,12 @@ hipError_t launch_kv_attn(const KvAttnArgs &args, hipStream_t s)
     a.units = (int32_t)p.units;
     a.split = p.split;
     a.wide = p.wide;
+    a.groups = (KvGroup *)((uint8_t *)a.ws + p.groups);
+    if (a.b.n_seqs > 64) {
+        hipLaunchKernelGGL(k_kv_list, dim3(1), dim3(1024), 0, s, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
     if (p.wide_items) {
         const dim3 g((unsigned)p.wide_items), block(KW_WAVES * 64);
         switch (a.hd * (a.c.type == DMOE_KV_E4M3 ? -1 : 1)) {

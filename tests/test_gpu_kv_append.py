@@ -103,6 +103,7 @@ GROUPS = {
     "across": [(30, 5)], "long": [(17, 300)],
     "ragged": [(5, 3), (0, 0), (31, 1), (32, 40), (700, 1), (64, 32), (0, 1), (63, 70), (96, 9), (33, 0), (40, 17)],
     "singles": [(i * 7, 1) for i in range(70)],
+    "many": [(i * 37 % 700, i % 6) for i in range(150)], "rows": [(i % 50, 40) for i in range(70)],
 }
 SHAPES = [  # n_head, n_head_kv, head_dim, rotary_dim, qk_norm, page_tokens
     (32, 4, 128, 64, True, 64), (5, 1, 64, 64, True, 32), (6, 3, 64, 20, False, 96), (3, 3, 128, 128, True, 256),
@@ -131,6 +132,16 @@ def _one(ctx, kvtype, group, nh, nkv, hd, rd, qk, T, scale=1.0, extra=3):
     gains = [rng.uniform(0.5, 1.5, hd).astype(np.float32) if qk else None for _ in range(2)]
     q, after = _run(ctx, batch, cache, qkv, nh, rd, qk, gains)
     _check(batch, cache, after, q, qkv, nh, rd, gains)
+
+
+@pytest.mark.parametrize("kvtype", ["f16", "e4m3"])
+def test_append_thousands(ctx, kvtype):
+    """More sequences than one look of 64 times 64 finds, half of them with a row."""
+    GROUPS["thousands"] = [(i * 7 % 60, (i * 5 + i // 64) % 2) for i in range(4300)]
+    try:
+        _one(ctx, kvtype, "thousands", 2, 1, 64, 32, False, 32)
+    finally:
+        del GROUPS["thousands"]
 
 
 @pytest.mark.parametrize("scale", [1e-30, 1e-14, 1e-3, 3e3, 1e16, 1e30])

@@ -71,6 +71,7 @@ GROUPS = {
     "full": [(10, 2300)],                            # more workgroups than start at once
     "padded": [(3000, 40)],                          # fewer rows than the buffers hold
     "many": [(i * 397 % 1700, i % 6) for i in range(150)],
+    "crowd": [(i * 13 % 800, 1) for i in range(70)] + [(10, 1500), (0, 0), (3000, 33), (2, 200)] + [(i * 41 % 900, i % 3) for i in range(70)],
 }
 
 
@@ -241,3 +242,15 @@ def test_rows_of_an_earlier_sequence(ctx, n):
     ref, top_v, top_s = attend(batch, c0, q0, 1)
     tol = R.attend_tolerance(top_v, top_s, hd, 900 + n)
     assert max(np.abs(o0 - ref).max(), np.abs(o1 - ref).max()) <= tol
+
+
+@pytest.mark.parametrize("kvtype", ["f16", "e4m3"])
+def test_thousands_of_sequences(ctx, kvtype):
+    """More sequences than one look of 64 times 64 finds, half of them with a row."""
+    nh, nkv, hd, T = 2, 1, 64, 32
+    print(f"case: attn {kvtype}, 4300 sequences", flush=True)
+    batch = R.Batch([(i * 7 % 60, (i * 5 + i // 64) % 2) for i in range(4299)] + [(900, 3)], T, seed=22, extra=2)
+    cache = R.Cache(kvtype, batch.n_pages, nkv, hd, T, seed=23)
+    _poison(batch, cache)
+    q = _q(batch, nh, hd, 24)
+    _check(batch, cache, q, 1, _run(ctx, batch, cache, q, 1))
